@@ -22,6 +22,22 @@ class DeviceInfo(C.Structure):
     _fields_ = [("name", C.c_char * 256), ("major", C.c_int), ("minor", C.c_int), ("total_memory", C.c_size_t)]
 
 
+class KVInt8Cache(C.Structure):
+    """Layout of ng_kv_int8_cache in include/kv_cache.h."""
+
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("num_pages", _i),
+                ("num_kv_heads", _i), ("head_dim", _i), ("page_size", _i)]
+
+
+class KVPages(C.Structure):
+    """Layout of ng_kv_pages in include/kv_cache.h."""
+
+    _fields_ = [("table", _vp), ("refs", _vp), ("max_seqs", _i), ("max_pages", _i), ("num_pages", _i),
+                ("page_size", _i)]
+
+
+_kvp, _pgp = C.POINTER(KVInt8Cache), C.POINTER(KVPages)
+
 # name -> (restype, argtypes). One entry per declaration in include/*.h.
 SIGNATURES: dict[str, tuple] = {
     # memory.h
@@ -101,6 +117,20 @@ SIGNATURES: dict[str, tuple] = {
     "ng_gemm_int8_add": (_i, [_vp, _vp, _cvp, _cvp, _cvp, _cvp, _i, _i, _i]),
     "ng_rmsnorm_qkv_rope_int8": (_i, [_vp, _vp, _vp, _vp, _cvp, _cvp, _f, C.POINTER(_cvp), C.POINTER(_cvp), _ip, _i,
                                       _i, _i, _i, _i, _f]),
+    # kv_cache.h
+    "ng_kv_int8_append": (_i, [_kvp, _cvp, _cvp, _cvp, _cvp, _cvp, _i, _i, _i, _i, _vp]),
+    "ng_bf16_kv_int8_append": (_i, [_kvp, _cvp, _cvp, _cvp, _cvp, _cvp, _i, _i, _i, _i, _vp]),
+    "ng_kv_int8_read": (_i, [_kvp, _vp, _vp, _cvp, _cvp, _cvp, _i, _i, _i, _i]),
+    "ng_bf16_kv_int8_read": (_i, [_kvp, _vp, _vp, _cvp, _cvp, _cvp, _i, _i, _i, _i]),
+    "ng_kv_int8_attention_workspace": (_sz, [_kvp, _i, _i, _i, _i]),
+    "ng_kv_int8_attention": (_i, [_vp, _cvp, _kvp, _cvp, _cvp, _cvp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _sz]),
+    "ng_bf16_kv_int8_attention": (_i, [_vp, _cvp, _kvp, _cvp, _cvp, _cvp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp,
+                                       _sz]),
+    "ng_kv_int8_copy_pages": (_i, [_kvp, _i, _cvp, _cvp, _i]),
+    "ng_kv_pages_grow": (_i, [_pgp, _cvp, _cvp, _vp, _vp, _vp]),
+    "ng_kv_pages_fork": (_i, [_pgp, _vp, _cvp, _cvp, _vp]),
+    "ng_kv_pages_free": (_i, [_pgp, _cvp, _cvp]),
+    "ng_kv_pages_compact": (_i, [_pgp, _vp, _vp, _i, _vp]),
 }
 
 _LIB = None
