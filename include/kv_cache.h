@@ -101,7 +101,8 @@ int ng_bf16_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const 
  * workspace of their own (16-byte aligned).
  * num_q_heads is a multiple of num_kv_heads; q and out are 16-byte aligned;
  * softmax_scale is finite and >= 0; window and sinks are >= 0. Scores, sums and
- * the output are held in 32 bits, weights are rounded to 11 bits. */
+ * the output are held in 32 bits; a weight times its page's V scale is rounded
+ * to 11 bits, and to 2^-25 of the largest V scale that the query sees. */
 size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, int num_q_heads, int batch, int max_q_len,
                                       int max_kv_len);
 int ng_kv_int8_attention(void* out, const void* q, const ng_kv_int8_cache* cache, const void* cu_q,

@@ -2,12 +2,36 @@
 // layout: kv_cache.hpp).
 //
 // With a page's scales k_s, v_s, codes k, v and x_j = c k_s (q . k_j):
-//   out = sum_j exp(x_j - m) v_s v_j / sum_j exp(x_j - m),  m a running maximum
-// of the visible x_j, sums in 32 bits. One pass over the cache.
+//   out = sum_j 2^(x_j - m) v_s v_j / sum_j 2^(x_j - m),  m a running maximum
+// of the visible x_j (c holds log2 e), sums in 32 bits. One pass over the cache.
+//
+// Both products run on the matrix cores with the codes as exact fp16 integers:
+//   S^T = K Q^T: rows are tokens, columns queries; the scale of a token's page
+//     multiplies the 32-bit sums.
+//   O^T = V^T P^T: a lane of S^T holds 4 tokens of one query, which are 4 of the 8
+//     values of its second operand, so P goes from one product into the next
+//     without leaving its lane. P's entries are 2^(x - m) v_s / u, u the
+//     largest v_s that the row has met (the sums are rescaled when it grows, as
+//     they are when m does): at most 1, rounded to fp16 (11 bits) once.
+// The queries of all heads that share a key/value head, and of several tokens,
+// are the columns: row r of a sequence and key/value head is head r % group of
+// its token r / group.
+//
+// bf16 queries become fp16 times a power of two of their row, which loses
+// nothing of elements within 2^-14 of the row's largest, and at most 2^-25 of
+// that largest for the others.
 #include "kv_cache.hpp"
+
+#include <algorithm>
 
 namespace ng {
 namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLeastUnit = 0x1p-126f;  // u of a row that has met nothing; its reciprocal is finite
 
 struct AttnArgs {
     const int* cu;
@@ -16,79 +40,435 @@ struct AttnArgs {
     int max_pages, total, hq, group;
     float scale;  // softmax_scale log2(e)
     int window, sinks;
+    int splits, chunk;  // slices of a sequence that there is room for; tiles of a slice
+    float* part;        // their outputs [splits][total hq][D], then (m, l) [splits][total hq]
 };
 
-// One wave per query row and head, a token per lane.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void kv_attention_row_kernel(uint16_t* out, const uint16_t* q, KvView kv, AttnArgs a) {
-    constexpr int C = D / 64;
-    __shared__ float s_q[D], s_p[64];
-    __shared__ int s_page[64];
-    const int b = blockIdx.y, hh = blockIdx.z, h = hh / a.group, lane = threadIdx.x;
-    const KvRows rows = kv_rows(a.cu, b, a.total);
-    const int ps = 1 << kv.ps_log2;
-    const int len = min(max(a.lens[b], 0), a.max_pages << kv.ps_log2);
-    const int lost = max(a.lens[b], 0) - len;  // tokens past the table are not there
-    for (int i = blockIdx.x; i < rows.count; i += gridDim.x) {
-        const int p = len + lost - rows.count + i;
-        const size_t ro = (static_cast<size_t>(rows.first + i) * a.hq + hh) * D;
-        for (int d = lane; d < D; d += 64) s_q[d] = to_f32<T>(q[ro + d]);
-        __syncthreads();
-        float m = -__builtin_inff(), l = 0.0f, acc[C];
+// Two int8 codes (bytes SEL0 and SEL1 of one dword) as exact fp16 values: biased
+// to u = q + 128, placed under an fp16 exponent of 2^10, 1152 subtracted.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t biased) {
+    const f16x2 bias = {static_cast<f16>(-1152.0f), static_cast<f16>(-1152.0f)};
+    const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, biased, SEL)) + bias;
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ f16x8 codes8(uint32_t lo, uint32_t hi) {
+    const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+    return __builtin_bit_cast(f16x8, u32x4{codes2<0x04010400u>(a), codes2<0x04030402u>(a), codes2<0x04010400u>(b),
+                                           codes2<0x04030402u>(b)});
+}
+
+// The tokens that a run of queries (positions p0 .. p1) sees, in tiles of 64:
+// `lead` tiles from 0 on for the first tokens, then those from tile `from` on.
+struct Tiles {
+    int lead, from, count;
+    __device__ __forceinline__ int tile(int i) const { return i < lead ? i : from + i - lead; }
+};
+__device__ __forceinline__ Tiles tiles_seen(int p0, int p1, int len, int window, int sinks) {
+    const int end = (min(p1 + 1, len) + 63) >> 6;
+    if (end <= 0) return {0, 0, 0};
+    if (window == 0) return {0, 0, end};
+    const int from = min(max(p0 - window + 1, 0) >> 6, end);
+    const int lead = min((min(sinks, len) + 63) >> 6, from);
+    return {lead, from, lead + end - from};
+}
+
+// How a row tile's tiles are shared out: slices of `chunk` tiles.
+struct Slices {
+    int chunk, count;
+};
+__device__ __forceinline__ Slices slices(const AttnArgs& a, int tiles) {
+    const int chunk = max(a.chunk, (tiles + a.splits - 1) / a.splits);
+    return {chunk, max((tiles + chunk - 1) / chunk, 1)};
+}
+
+// One sequence as a block sees it.
+struct Seq {
+    KvRows rows;
+    int last;   // position of its last query
+    int len;    // tokens that the table can hold of it
+    const int* table;
+};
+__device__ __forceinline__ Seq sequence(const AttnArgs& a, const KvView& kv, int b) {
+    Seq s;
+    s.rows = kv_rows(a.cu, b, a.total);
+    const int n = min(max(load_uniform(a.lens + b), 0), 1 << 30);
+    s.last = n - 1;
+    s.len = min(n, a.max_pages << kv.ps_log2);
+    s.table = a.table + static_cast<size_t>(b) * a.max_pages;
+    return s;
+}
+
+// A 16-token sub-block of a head: byte offset of its codes, index of its scales,
+// and whether there is such a page (if not, both name the first one, whose
+// memory is there to be read).
+struct Sub {
+    size_t codes, scale;
+    bool there;
+};
+__device__ __forceinline__ Sub sub_block(const KvView& kv, const Seq& s, int h, int token, int D) {
+    int page = token < s.len ? load_uniform(s.table + (token >> kv.ps_log2)) : -1;
+    const bool there = page >= 0 && page < kv.num_pages;
+    page = there ? page : 0;
+    const size_t ph = static_cast<size_t>(page) * kv.hkv + h;
+    return {((ph << kv.ps_log2) + (token & ((1 << kv.ps_log2) - 1))) * D, ph, there};
+}
+
+// Maximum and sum over the four lanes that hold a column of a 16 x 16 tile.
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v += __shfl_xor(v, 16, kWave);
+    return v + __shfl_xor(v, 32, kWave);
+}
+
+// 2^(m - to) where to >= m may be -inf (nothing seen yet on either side).
+__device__ __forceinline__ float decay(float m, float to) {
+    return __builtin_amdgcn_exp2f(m - (to == kNegInf ? 0.0f : to));
+}
+
+// Queries as operands: lane (column, kg) holds d = 64 c + 16 kg + 8 j + 0 .. 7 of its row in q[c][j].
+// Returns the factor that undoes bf16's scaling.
+template <typename T, int C>
+__device__ __forceinline__ float load_queries(const uint16_t* row, bool real, int kg, f16x8 (&q)[C][2]) {
+    u32x4 raw[C][2];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = 0.0f;
-        const int end = min(p, len - 1);
-        for (int j0 = 0; j0 <= end; j0 += 64) {
-            const int j = j0 + lane;
-            bool seen = j <= end && (a.window == 0 || j > p - a.window || j < a.sinks);
-            const int page = seen ? a.table[static_cast<size_t>(b) * a.max_pages + (j >> kv.ps_log2)] : -1;
-            seen = page >= 0 && page < kv.num_pages;
-            float x = -__builtin_inff(), vs = 0.0f;
-            const int slot = j & (ps - 1);
-            if (seen) {
-                const size_t ph = static_cast<size_t>(page) * kv.hkv + h;
-                const uint8_t* kc = kv.kc + ph * (static_cast<size_t>(ps) * D) + (slot >> 4) * 16 * D + (slot & 15) * 16;
-                float s = 0.0f;
-                for (int d = 0; d < D; ++d)
-                    s += s_q[d] * static_cast<float>(static_cast<int8_t>(kc[(d >> 6) * 1024 + ((d >> 4) & 3) * 256 + (d & 15)]));
-                x = s * (kv.ks[ph] * a.scale);
-                vs = kv.vs[ph];
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) raw[c][j] = real ? ld16(row + 64 * c + 16 * kg + 8 * j) : u32x4{0, 0, 0, 0};
+    if constexpr (__is_same(T, f16)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) q[c][j] = __builtin_bit_cast(f16x8, raw[c][j]);
+        return 1.0f;
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) m = absmax_bits8(raw[c][j], m);
+        m = umax32(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, kWave)));
+        m = umax32(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, kWave)));
+        const int e = max(static_cast<int>(m >> 7), 1) - 127;  // 2^e <= largest < 2^(e + 1)
+        const float f = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x[8];
+                unpack8<bf16>(raw[c][j], x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= f;
+                q[c][j] = __builtin_bit_cast(f16x8, pack8<f16>(x));
             }
-            const float mn = fmaxf(m, wave_max_f32(x));
-            const float ms = mn == -__builtin_inff() ? 0.0f : mn;
-            const float e = seen ? __builtin_amdgcn_exp2f(x - ms) : 0.0f, f = __builtin_amdgcn_exp2f(m - ms);
-            l = l * f + wave_sum_f32(e);
-            m = mn;
-            s_p[lane] = e * vs;
-            s_page[lane] = seen ? page : -1;
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] *= f;
-            for (int t = 0; t < 64 && j0 + t <= end; ++t) {
-                if (s_page[t] < 0) continue;
-                const int sl = (j0 + t) & (ps - 1), tt = sl & 15;
-                const uint8_t* vc = kv.vc + (static_cast<size_t>(s_page[t]) * kv.hkv + h) * (static_cast<size_t>(ps) * D) +
-                                    (sl >> 4) * 16 * D;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int kg = lane >> 4, i4 = (lane >> 2) & 3, r = lane & 3;
-                    acc[c] += s_p[t] * static_cast<float>(static_cast<int8_t>(
-                                           vc[c * 1024 + (kg * 16 + (tt >> 2) * 4 + r) * 16 + i4 * 4 + (tt & 3)]));
-                }
-            }
-            __syncthreads();
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-        for (int c = 0; c < C; ++c) out[ro + 64 * c + lane] = from_f32<T>(acc[c] * inv);
+        return __builtin_ldexpf(1.0f, e);
     }
 }
 
+// Few queries to a sequence: bound by reading the cache. A block of four waves
+// takes up to 16 rows and a slice of the tokens; a wave every fourth tile of
+// 16 NB tokens, straight from memory into registers: K's codes of the next
+// tile are requested when this tile's are used up, then V's, so that half a
+// tile is always on its way. The waves' results are joined in LDS.
+// Grid: slices, key/value heads x row tiles (strided over), batch.
+constexpr int kDecodeWaves = 4;
+
+template <typename T, int D, int NB>
+__global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_t* out, const uint16_t* q, KvView kv,
+                                                                         AttnArgs a) {
+    constexpr int C = D / 64;
+    constexpr int kPer = 4 / NB;  // steps of a 64-token tile
+    __shared__ f32x4 s_o[kDecodeWaves - 1][D / 4][16];
+    __shared__ float s_m[kDecodeWaves][16], s_l[kDecodeWaves][16];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 15, kg = lane >> 4;
+    const uint32_t koff = lane * 16, voff = (16 * (col >> 2) + 4 * kg + (col & 3)) * 16;
+    const Seq s = sequence(a, kv, blockIdx.z);
+    const int h = blockIdx.y % kv.hkv;
+    const int R = s.rows.count * a.group;
+    for (int r0 = blockIdx.y / kv.hkv * 16; r0 < R; r0 += static_cast<int>(gridDim.y) / kv.hkv * 16) {
+        const int r = r0 + col;
+        const bool real = r < R;
+        const int i = r / a.group;
+        const int p = real ? s.last - s.rows.count + 1 + i : -1;
+        const int p0 = s.last - s.rows.count + 1 + r0 / a.group;
+        const int p1 = s.last - s.rows.count + 1 + min(r0 + 15, R - 1) / a.group;
+        const Tiles tl = tiles_seen(p0, p1, s.len, a.window, a.sinks);
+        const Slices sl = slices(a, tl.count);
+        if (static_cast<int>(blockIdx.x) >= sl.count) continue;
+        const size_t row = static_cast<size_t>(s.rows.first + i) * a.hq + h * a.group + (r - i * a.group);
+        f16x8 qf[C][2];
+        const float unscale = load_queries<T, C>(q + row * D, real, kg, qf);
+
+        const int v0 = static_cast<int>(blockIdx.x) * sl.chunk, v1 = min(v0 + sl.chunk, tl.count);
+        const int steps = max(v1 - v0, 0) * kPer;  // of the block; wave w takes step w, w + 4, ...
+        const auto token_of = [&](int step) { return tl.tile(v0 + step / kPer) * 64 + step % kPer * (16 * NB); };
+        u32x4 kr[NB][C], vr[NB][C];
+        Sub sub[NB], nsub[NB];
+        const auto find = [&](int step, Sub (&x)[NB]) {
+            const int t0 = token_of(step);
+#pragma unroll
+            for (int t = 0; t < NB; ++t) x[t] = sub_block(kv, s, h, t0 + 16 * t, D);
+        };
+        const auto load_k = [&](const Sub (&x)[NB]) {
+#pragma unroll
+            for (int t = 0; t < NB; ++t)
+#pragma unroll
+                for (int c = 0; c < C; ++c) kr[t][c] = ld16_stream(kv.kc + x[t].codes + 1024 * c + koff);
+        };
+        const auto load_v = [&](const Sub (&x)[NB]) {
+#pragma unroll
+            for (int t = 0; t < NB; ++t)
+#pragma unroll
+                for (int c = 0; c < C; ++c) vr[t][c] = ld16_stream(kv.vc + x[t].codes + 1024 * c + voff);
+        };
+        float m = kNegInf, l = 0.0f, u = kLeastUnit;
+        f32x4 acc[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        int step = wave;
+        if (step < steps) {
+            find(step, sub);
+            load_k(sub);
+            load_v(sub);
+        }
+        for (; step < steps; step += kDecodeWaves) {
+            const bool more = step + kDecodeWaves < steps;
+            if (more) find(step + kDecodeWaves, nsub);
+            float ks[NB], vs[NB];
+#pragma unroll
+            for (int t = 0; t < NB; ++t) ks[t] = load_uniform(kv.ks + sub[t].scale), vs[t] = load_uniform(kv.vs + sub[t].scale);
+            f32x4 x[NB];
+#pragma unroll
+            for (int t = 0; t < NB; ++t) {
+                x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][0], kr[t][c][1]), qf[c][0], x[t], 0, 0, 0);
+                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][2], kr[t][c][3]), qf[c][1], x[t], 0, 0, 0);
+                }
+            }
+            if (more) load_k(nsub);
+            // Scores; those of tokens that a row does not see become -inf.
+            const int t0 = token_of(step);
+            bool whole = t0 + 16 * NB - 1 <= p0 && t0 + 16 * NB <= s.len &&
+                         (a.window == 0 || t0 > p1 - a.window || t0 + 16 * NB <= a.sinks);
+#pragma unroll
+            for (int t = 0; t < NB; ++t) whole = whole && sub[t].there;
+            float sc[NB][4];
+#pragma unroll
+            for (int t = 0; t < NB; ++t) {
+                const float f = ks[t] * a.scale * unscale;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[t][e] = x[t][e] * f;
+            }
+            float un = 0.0f;  // the largest v_s of pages with a token that the row sees
+            if (whole) {
+#pragma unroll
+                for (int t = 0; t < NB; ++t) un = fmaxf(un, vs[t]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < NB; ++t) {
+                    bool some = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = t0 + 16 * t + 4 * kg + e;
+                        const bool seen = sub[t].there & (j <= p) & (j < s.len) &
+                                          ((a.window == 0) | (j > p - a.window) | (j < a.sinks));
+                        sc[t][e] = seen ? sc[t][e] : kNegInf;
+                        some |= seen;
+                    }
+                    vs[t] = some ? vs[t] : 0.0f;
+                    un = fmaxf(un, vs[t]);
+                }
+                un = col_max(un);
+            }
+            un = fmaxf(un, u);
+            float mx = m;
+#pragma unroll
+            for (int t = 0; t < NB; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
+            mx = col_max(mx);
+            const float base = mx == kNegInf ? 0.0f : mx;
+            const float down = decay(m, mx);
+            l *= down;
+            const float inv_u = __builtin_amdgcn_rcpf(un);
+            const float fade = un > u ? down * (u * inv_u) : down;
+            if (__any(fade != 1.0f)) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[c][j] *= fade;
+            }
+            m = mx;
+            u = un;
+            uint32_t pp[NB][2];
+#pragma unroll
+            for (int t = 0; t < NB; ++t) {
+                const float f = vs[t] * inv_u;
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(sc[t][e] - base);
+                    l += w[e];
+                    w[e] *= f;
+                }
+                pp[t][0] = pack2<f16>(w[0], w[1]);
+                pp[t][1] = pack2<f16>(w[2], w[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < NB; t += 2) {
+                const f16x8 pb = __builtin_bit_cast(f16x8, u32x4{pp[t][0], pp[t][1], pp[t + 1][0], pp[t + 1][1]});
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vr[t][c][j], vr[t + 1][c][j]), pb,
+                                                                           acc[c][j], 0, 0, 0);
+            }
+            if (more) load_v(nsub);
+#pragma unroll
+            for (int t = 0; t < NB; ++t) sub[t] = nsub[t];
+        }
+        l = col_sum(l);
+        // Join the waves: lane (column, kg) of each holds d = 64 c + 16 kg + 4 j + e.
+        if (kg == 0) {
+            s_m[wave][col] = m;
+            s_l[wave][col] = l;
+        }
+        __syncthreads();
+        float M = s_m[0][col];
+#pragma unroll
+        for (int w = 1; w < kDecodeWaves; ++w) M = fmaxf(M, s_m[w][col]);
+        float L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDecodeWaves; ++w) L += s_l[w][col] * decay(s_m[w][col], M);
+        const float f = decay(m, M) * u;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[c][j] *= f;
+                if (wave > 0) s_o[wave - 1][16 * c + 4 * kg + j][col] = acc[c][j];
+            }
+        __syncthreads();
+        if (wave == 0 && real) {
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const size_t all = static_cast<size_t>(a.total) * a.hq;
+            const size_t slot = blockIdx.x * all + row;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float o[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int w = 0; w < kDecodeWaves - 1; ++w) acc[c][j] += s_o[w][16 * c + 4 * kg + j][col];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * j + e] = acc[c][j][e] * inv;
+                }
+                if (sl.count > 1) {
+                    float* to = a.part + slot * D + 64 * c + 16 * kg;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<f32x4*>(to + 4 * j) = f32x4{o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]};
+                } else {
+                    uint16_t* to = out + row * D + 64 * c + 16 * kg;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = o[8 * j + e];
+                        st16(to + 8 * j, pack8<T>(y));
+                    }
+                }
+            }
+            if (sl.count > 1 && kg == 0) {
+                float* ml = a.part + a.splits * all * D + slot * 2;
+                ml[0] = M;
+                ml[1] = L;
+            }
+        }
+        __syncthreads();  // LDS is free for the next row tile
+    }
+}
+
+// Joins the slices of a row: out = sum_s l_s 2^(m_s - M) o_s / sum_s l_s 2^(m_s - M),
+// added in slice order. A wave per row; rows of one slice are done already.
+// Grid: rows of a sequence (strided over), batch.
 template <typename T, int D>
-int launch_attention(const dim3& grid, void* out, const void* q, const KvView& kv, const AttnArgs& a) {
-    kv_attention_row_kernel<T, D><<<grid, dim3(64), 0, stream()>>>(static_cast<uint16_t*>(out),
-                                                                  static_cast<const uint16_t*>(q), kv, a);
-    return 0;
+__global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv, AttnArgs a) {
+    constexpr int C = D / 64;
+    const Seq s = sequence(a, kv, blockIdx.y);
+    const int lane = threadIdx.x;
+    const size_t all = static_cast<size_t>(a.total) * a.hq;
+    for (int rr = blockIdx.x; rr < s.rows.count * a.hq; rr += gridDim.x) {
+        const int i = rr / a.hq, hh = rr - i * a.hq;
+        const int r = i * a.group + hh % a.group, r0 = r & ~15, R = s.rows.count * a.group;
+        const int p0 = s.last - s.rows.count + 1 + r0 / a.group;
+        const int p1 = s.last - s.rows.count + 1 + min(r0 + 15, R - 1) / a.group;
+        const int n = slices(a, tiles_seen(p0, p1, s.len, a.window, a.sinks).count).count;
+        if (n == 1) continue;
+        const size_t row = static_cast<size_t>(s.rows.first) * a.hq + rr;
+        const float* ml = a.part + a.splits * all * D + row * 2;
+        float M = kNegInf;
+        for (int x = lane; x < n; x += kWave) M = fmaxf(M, ml[x * all * 2]);
+        M = wave_max_f32(M);
+        float L = 0.0f, o[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = 0.0f;
+        for (int x = 0; x < n; ++x) {
+            const float w = ml[x * all * 2 + 1] * decay(ml[x * all * 2], M);
+            L += w;
+#pragma unroll
+            for (int c = 0; c < C; ++c) o[c] += w * a.part[(x * all + row) * D + 64 * c + lane];
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int c = 0; c < C; ++c) out[row * D + 64 * c + lane] = from_f32<T>(o[c] * inv);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------
+
+// Slices worth having: enough blocks for kBlocksWanted, at least kTilesLeast
+// tiles in each.
+constexpr int kBlocksWanted = 1024, kTilesLeast = 8;
+struct Plan {
+    int row_tiles, splits, chunk;
+};
+Plan plan(int hkv, int group, int batch, int max_q, int max_kv) {
+    Plan p;
+    p.row_tiles = static_cast<int>((static_cast<long long>(max_q) * group + 15) / 16);
+    const int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
+    const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
+    const long long want = (kBlocksWanted + blocks - 1) / blocks;
+    const int most = std::max(tiles / kTilesLeast, 1);
+    p.splits = static_cast<int>(std::min<long long>(want, most));
+    p.chunk = (tiles + p.splits - 1) / p.splits;
+    p.splits = (tiles + p.chunk - 1) / p.chunk;
+    return p;
+}
+
+size_t slice_bytes(size_t rows, int D) { return rows * (D + 2) * sizeof(float); }
+
+template <typename T, int D>
+void launch_attention(const Plan& p, int batch, uint16_t* out, const uint16_t* q, const KvView& kv, const AttnArgs& a,
+                      int max_q) {
+    constexpr int NB = D <= 128 ? 4 : 2;
+    const int y = std::min(p.row_tiles, std::max(1, 65535 / kv.hkv)) * kv.hkv;
+    kv_decode_kernel<T, D, NB><<<dim3(p.splits, y, batch), dim3(kDecodeWaves * kWave), 0, stream()>>>(out, q, kv, a);
+    if (p.splits > 1) {
+        const long long rows = static_cast<long long>(max_q) * a.hq;
+        kv_join_kernel<T, D><<<dim3(static_cast<unsigned>(std::min<long long>(rows, 1 << 20)), batch), dim3(kWave), 0,
+                               stream()>>>(out, kv, a);
+    }
 }
 
 template <typename T>
@@ -104,16 +484,29 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
     NG_REQUIRE(__builtin_isfinite(scale) && scale >= 0.0f, "%s: softmax_scale must be finite and >= 0", name);
     NG_REQUIRE(window >= 0 && sinks >= 0, "%s: window and sinks must be >= 0", name);
     NG_REQUIRE(aligned16(out) && aligned16(q) && aligned16(workspace), "%s: pointers must be 16-byte aligned", name);
-    const AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table),
-                     max_pages, total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f,
-                     min(window, 1 << 30), sinks};
-    const dim3 grid(min(max_q, 65535), batch, hq);
+    NG_REQUIRE(static_cast<long long>(total) * hq <= (1ll << 30), "%s: more than 2^30 query rows", name);
+    max_q = std::min(max_q, total);
+    AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
+               total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,
+               1, 1, static_cast<float*>(workspace)};
+    Plan p = plan(cache->num_kv_heads, a.group, batch, max_q, max_kv);
+    const size_t rows = static_cast<size_t>(total) * hq;
+    const size_t room = workspace == nullptr ? 0 : workspace_bytes / slice_bytes(rows, cache->head_dim);
+    if (room < static_cast<size_t>(p.splits)) {
+        const int tiles = p.chunk * p.splits;
+        p.splits = std::max<int>(static_cast<int>(room), 1);
+        p.chunk = (tiles + p.splits - 1) / p.splits;
+    }
+    a.splits = p.splits;
+    a.chunk = p.chunk;
     const KvView kv = kv_view(*cache);
+    uint16_t* o = static_cast<uint16_t*>(out);
+    const uint16_t* x = static_cast<const uint16_t*>(q);
     switch (cache->head_dim) {
-        case 64: launch_attention<T, 64>(grid, out, q, kv, a); break;
-        case 128: launch_attention<T, 128>(grid, out, q, kv, a); break;
-        case 192: launch_attention<T, 192>(grid, out, q, kv, a); break;
-        default: launch_attention<T, 256>(grid, out, q, kv, a); break;
+        case 64: launch_attention<T, 64>(p, batch, o, x, kv, a, max_q); break;
+        case 128: launch_attention<T, 128>(p, batch, o, x, kv, a, max_q); break;
+        case 192: launch_attention<T, 192>(p, batch, o, x, kv, a, max_q); break;
+        default: launch_attention<T, 256>(p, batch, o, x, kv, a, max_q); break;
     }
     NG_CHECK_LAUNCH(name);
     return 0;
@@ -126,7 +519,12 @@ using namespace ng;
 
 extern "C" size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, int num_q_heads, int batch,
                                                  int max_q_len, int max_kv_len) {
-    return 0;
+    if (cache == nullptr || cache->num_kv_heads <= 0 || !kv_head_dim_ok(cache->head_dim) || num_q_heads <= 0 ||
+        num_q_heads % cache->num_kv_heads != 0 || batch <= 0 || max_q_len <= 0 || max_kv_len <= 0)
+        return 0;
+    const Plan p = plan(cache->num_kv_heads, num_q_heads / cache->num_kv_heads, batch, max_q_len, max_kv_len);
+    if (p.splits <= 1) return 0;
+    return p.splits * slice_bytes(static_cast<size_t>(batch) * max_q_len * num_q_heads, cache->head_dim);
 }
 
 extern "C" int ng_kv_int8_attention(void* out, const void* q, const ng_kv_int8_cache* cache, const void* cu_q,

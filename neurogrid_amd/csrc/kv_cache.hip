@@ -60,7 +60,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
     const int waves = blockDim.x / kWave;
     const int ps = 1 << kv.ps_log2, cap = max_pages << kv.ps_log2;
     const KvRows rows = kv_rows(cu, b, total);
-    const int ctx = min(max(ctx_lens[b], 0), cap);
+    const int ctx = min(max(load_uniform(ctx_lens + b), 0), cap);
     const int n = min(rows.count, cap - ctx);
     const bool counts = dropped != nullptr && blockIdx.z == 0 && threadIdx.x == 0;
     if (counts && blockIdx.x == 0 && rows.count > n) atomicAdd(dropped, rows.count - n);
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
     for (int pg = (ctx >> kv.ps_log2) + blockIdx.x; pg <= last; pg += gridDim.x) {
         const int t0 = pg << kv.ps_log2;
         const int lo = max(ctx - t0, 0), hi = min(ctx + n - t0, ps);  // slots lo .. hi - 1 are new
-        const int page = table[static_cast<size_t>(b) * max_pages + pg];
+        const int page = load_uniform(table + static_cast<size_t>(b) * max_pages + pg);
         if (page < 0 || page >= kv.num_pages) {
             if (counts) atomicAdd(dropped, hi - lo);
             continue;
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(512) void kv_read_kernel(KvView kv, uint16_t* k, ui
     const int ps = 1 << kv.ps_log2;
     const KvRows rows = kv_rows(cu, b, total);
     if (rows.count == 0) return;
-    const int start = min(max(starts[b], 0), 1 << 30);
+    const int start = min(max(load_uniform(starts + b), 0), 1 << 30);
     uint16_t* x = (is_v ? v : k) + static_cast<size_t>(rows.first) * kv.hkv * D + static_cast<size_t>(h) * D;
     const int kg = lane >> 4, t = lane & 15;
     const uint32_t sel = quad_selector(lane);
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(512) void kv_read_kernel(KvView kv, uint16_t* k, ui
         const int lo = max(start - t0, 0), hi = min(start + rows.count - t0, ps);
         const int slot = wave * kSub + t;
         if (wave * kSub >= hi || wave * kSub + kSub <= lo) continue;
-        const int page = pg < max_pages ? table[static_cast<size_t>(b) * max_pages + pg] : -1;
+        const int page = pg < max_pages ? load_uniform(table + static_cast<size_t>(b) * max_pages + pg) : -1;
         const bool there = page >= 0 && page < kv.num_pages;
         const size_t ph = there ? static_cast<size_t>(page) * kv.hkv + h : 0;
         const uint8_t* mine = (is_v ? kv.vc : kv.kc) + ph * (static_cast<size_t>(ps) * D) +
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(512) void kv_read_kernel(KvView kv, uint16_t* k, ui
         u32x4 q[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) q[c] = there ? ld16(mine + 1024 * c) : u32x4{0, 0, 0, 0};
-        const float s = there ? (is_v ? kv.vs : kv.ks)[ph] : 0.0f;
+        const float s = there ? load_uniform((is_v ? kv.vs : kv.ks) + ph) : 0.0f;
         uint16_t* row = x + static_cast<ptrdiff_t>(t0 + slot - start) * kv.hkv * D + 16 * kg;
 #pragma unroll
         for (int c = 0; c < C; ++c) {

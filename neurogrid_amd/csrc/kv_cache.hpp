@@ -60,13 +60,21 @@ inline int kv_check_batch(const char* name, const ng_kv_int8_cache* c, const voi
     return 0;
 }
 
+// A load of memory that nothing writes while the kernel runs, at an address that
+// is the same for the whole wave: scalar, so that it does not queue behind the
+// vector loads in flight (a store to another array would otherwise forbid it).
+template <typename X>
+__device__ __forceinline__ X load_uniform(const X* p) {
+    return *(const __attribute__((address_space(4))) X*)(reinterpret_cast<uintptr_t>(p));
+}
+
 // Sequence b's rows of a packed batch, whatever cu holds.
 struct KvRows {
     int first, count;
 };
 __device__ __forceinline__ KvRows kv_rows(const int* cu, int b, int total) {
-    const int a = min(max(cu[b], 0), total);
-    return {a, max(min(cu[b + 1], total), a) - a};
+    const int a = min(max(load_uniform(cu + b), 0), total);
+    return {a, max(min(load_uniform(cu + b + 1), total), a) - a};
 }
 
 // 4 x 4 bytes transposed over the four lanes of a quad: byte e of lane r's
