@@ -29,6 +29,7 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLeastUnit = 0x1p-126f;  // u of a row that has met nothing; its reciprocal is finite
@@ -40,6 +41,7 @@ struct AttnArgs {
     int max_pages, total, hq, group;
     float scale;  // softmax_scale log2(e)
     int window, sinks;
+    int row_tile;       // rows that a block takes together
     int splits, chunk;  // slices of a sequence that there is room for; tiles of a slice
     float* part;        // their outputs [splits][total hq][D], then (m, l) [splits][total hq]
 };
@@ -129,41 +131,35 @@ __device__ __forceinline__ float decay(float m, float to) {
     return __builtin_amdgcn_exp2f(m - (to == kNegInf ? 0.0f : to));
 }
 
-// Queries as operands: lane (column, kg) holds d = 64 c + 16 kg + 8 j + 0 .. 7 of its row in q[c][j].
-// Returns the factor that undoes bf16's scaling.
-template <typename T, int C>
-__device__ __forceinline__ float load_queries(const uint16_t* row, bool real, int kg, f16x8 (&q)[C][2]) {
-    u32x4 raw[C][2];
+// N pieces of 8 elements of a query row, piece j at row + at(j), as fp16
+// operands; `lanes` (16 or 32) and its doubles reach the lanes that hold the rest
+// of the row. Returns the factor that undoes bf16's scaling.
+template <typename T, int N, int FROM, typename At>
+__device__ __forceinline__ float load_row(const uint16_t* row, bool real, At&& at, f16x8 (&q)[N]) {
+    u32x4 raw[N];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) raw[c][j] = real ? ld16(row + 64 * c + 16 * kg + 8 * j) : u32x4{0, 0, 0, 0};
+    for (int j = 0; j < N; ++j) raw[j] = real ? ld16(row + at(j)) : u32x4{0, 0, 0, 0};
     if constexpr (__is_same(T, f16)) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) q[c][j] = __builtin_bit_cast(f16x8, raw[c][j]);
+        for (int j = 0; j < N; ++j) q[j] = __builtin_bit_cast(f16x8, raw[j]);
         return 1.0f;
     } else {
         uint32_t m = 0;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int j = 0; j < N; ++j) m = absmax_bits8(raw[j], m);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) m = absmax_bits8(raw[c][j], m);
-        m = umax32(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, kWave)));
-        m = umax32(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, kWave)));
+        for (int off = FROM; off < kWave; off <<= 1)
+            m = umax32(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), off, kWave)));
         const int e = max(static_cast<int>(m >> 7), 1) - 127;  // 2^e <= largest < 2^(e + 1)
         const float f = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int j = 0; j < N; ++j) {
+            float x[8];
+            unpack8<bf16>(raw[j], x);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float x[8];
-                unpack8<bf16>(raw[c][j], x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= f;
-                q[c][j] = __builtin_bit_cast(f16x8, pack8<f16>(x));
-            }
+            for (int i = 0; i < 8; ++i) x[i] *= f;
+            q[j] = __builtin_bit_cast(f16x8, pack8<f16>(x));
+        }
         return __builtin_ldexpf(1.0f, e);
     }
 }
@@ -201,8 +197,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
         const Slices sl = slices(a, tl.count);
         if (static_cast<int>(blockIdx.x) >= sl.count) continue;
         const size_t row = static_cast<size_t>(s.rows.first + i) * a.hq + h * a.group + (r - i * a.group);
-        f16x8 qf[C][2];
-        const float unscale = load_queries<T, C>(q + row * D, real, kg, qf);
+        f16x8 qf[2 * C];  // piece 2 c + j: d = 64 c + 16 kg + 8 j + 0 .. 7
+        const float unscale = load_row<T, 2 * C, 16>(q + row * D, real, [&](int j) { return 64 * (j >> 1) + 16 * kg + 8 * (j & 1); }, qf);
 
         const int v0 = static_cast<int>(blockIdx.x) * sl.chunk, v1 = min(v0 + sl.chunk, tl.count);
         const int steps = max(v1 - v0, 0) * kPer;  // of the block; wave w takes step w, w + 4, ...
@@ -250,8 +246,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
                 x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][0], kr[t][c][1]), qf[c][0], x[t], 0, 0, 0);
-                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][2], kr[t][c][3]), qf[c][1], x[t], 0, 0, 0);
+                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][0], kr[t][c][1]), qf[2 * c], x[t], 0, 0, 0);
+                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kr[t][c][2], kr[t][c][3]), qf[2 * c + 1], x[t], 0, 0, 0);
                 }
             }
             if (more) load_k(nsub);
@@ -399,6 +395,244 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
     }
 }
 
+// Many queries to a sequence: bound by the matrix cores and the exponentials. A
+// block of four waves takes 128 rows, 32 a wave (32 x 32 x 16 MFMAs), and goes
+// through tiles of 64 tokens. A tile's codes become fp16 once a block, on their
+// way into LDS: while a tile is multiplied, the next one's codes, which arrived
+// in registers a tile earlier, are converted into the other half of LDS, and
+// the one after that is requested. Wave w brings sub-block w.
+//   K in LDS: 16-byte pieces (d / 8, token), V: (sub-block, g, position of d),
+//   a piece being the 8 tokens that lane half g of an MFMA's second operand
+//   holds, quads g and 2 + g. d = 64 c + 16 kg + 4 i + r stands at position
+//   64 c + 16 i + 4 kg + r, so that a wave's writes of one i are contiguous.
+// A row's maximum is raised only when a score passes it by 2^8 (weights up to
+// 2^8 then, exact all the same), so most tiles rescale nothing.
+// Grid: row tiles x key/value heads (the last rows, which see most, first; a
+// head's blocks next to each other in the same L2 where 8 divides the heads),
+// batch, slices.
+constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
+constexpr float kLazy = 8.0f;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_prompt_kernel(uint16_t* out,
+                                                                                          const uint16_t* q, KvView kv,
+                                                                                          AttnArgs a) {
+    constexpr int C = D / 64, kHalf = 64 * D * 2;  // bytes of a tile of K
+    __shared__ __align__(1024) uint8_t lds[2][2 * kHalf];
+    __shared__ __align__(16) float s_scale[2][2][4];  // of the sub-blocks: K's (< 0: no page), V's
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 31, g = lane >> 5;
+    const Seq s = sequence(a, kv, blockIdx.y);
+    const int h = blockIdx.x % kv.hkv;
+    const int R = s.rows.count * a.group, tiles = (R + kPromptRows - 1) / kPromptRows;
+    const int first = s.last - s.rows.count + 1;  // position of the first query
+    const int kput = ((2 * (lane >> 4)) * 64 + kSub * wave + (lane & 15)) * 16;
+    const int vput = ((2 * wave + ((lane >> 2) & 1)) * D + 4 * (lane >> 4) + (lane & 3)) * 16 + ((lane >> 3) & 1) * 8;
+    for (int rt = tiles - 1 - static_cast<int>(blockIdx.x) / kv.hkv; rt >= 0; rt -= static_cast<int>(gridDim.x) / kv.hkv) {
+        const int r0 = rt * kPromptRows;
+        const int p0 = first + r0 / a.group, p1 = first + min(r0 + kPromptRows - 1, R - 1) / a.group;
+        const Tiles tl = tiles_seen(p0, p1, s.len, a.window, a.sinks);
+        const Slices sl = slices(a, tl.count);
+        if (static_cast<int>(blockIdx.z) >= sl.count) continue;
+        const int v0 = static_cast<int>(blockIdx.z) * sl.chunk, v1 = min(v0 + sl.chunk, tl.count);
+        // The wave's rows and their positions.
+        const int rw = r0 + 32 * wave, r = rw + col;
+        const bool real = r < R;
+        const int i = r / a.group, p = real ? first + i : -1;
+        const int pw0 = first + rw / a.group, pw1 = rw < R ? first + min(rw + 31, R - 1) / a.group : -1;
+        const size_t row = static_cast<size_t>(s.rows.first + i) * a.hq + h * a.group + (r - i * a.group);
+        f16x8 qf[D / 16];
+        const float unscale = load_row<T, D / 16, 32>(q + row * D, real, [&](int j) { return 16 * j + 8 * g; }, qf);
+
+        u32x4 kr[C], vr[C];
+        float ks = -1.0f, vs = 0.0f;
+        Sub sub;
+        const auto find = [&](int v) { sub = sub_block(kv, s, h, tl.tile(v) * 64 + kSub * wave, D); };
+        const auto request = [&] {  // the sub-block in `sub`
+#pragma unroll
+            for (int c = 0; c < C; ++c) kr[c] = ld16(kv.kc + sub.codes + 1024 * c + 16 * lane);
+#pragma unroll
+            for (int c = 0; c < C; ++c) vr[c] = ld16(kv.vc + sub.codes + 1024 * c + 16 * lane);
+            ks = sub.there ? load_uniform(kv.ks + sub.scale) : -1.0f;
+            vs = sub.there ? load_uniform(kv.vs + sub.scale) : 0.0f;
+        };
+        const auto put = [&](int half) {  // what was requested, as fp16
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                uint8_t* k = lds[half] + kput + 8 * c * 1024;
+                *reinterpret_cast<f16x8*>(k) = codes8(kr[c][0], kr[c][1]);
+                *reinterpret_cast<f16x8*>(k + 1024) = codes8(kr[c][2], kr[c][3]);
+                uint8_t* v = lds[half] + kHalf + vput + c * 1024;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t b = vr[c][j] ^ 0x80808080u;
+                    *reinterpret_cast<u32x2*>(v + 256 * j) = u32x2{codes2<0x04010400u>(b), codes2<0x04030402u>(b)};
+                }
+            }
+            if (lane == 0) {
+                s_scale[half][0][wave] = ks;
+                s_scale[half][1][wave] = vs;
+            }
+        };
+
+        float m = kNegInf, l = 0.0f, u = kLeastUnit, inv_u = 0x1p126f;
+        f32x16 acc[D / 32];
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] = f32x16{};
+        if (v0 < v1) {
+            find(v0);
+            request();
+            put(0);
+            if (v0 + 1 < v1) {
+                find(v0 + 1);
+                request();
+            }
+            if (v0 + 2 < v1) find(v0 + 2);
+        }
+        __syncthreads();
+        for (int v = v0; v < v1; ++v) {
+            const int half = (v - v0) & 1;
+            const uint8_t *kb = lds[half] + (g * 64 + col) * 16, *vb = lds[half] + kHalf + (g * D + col) * 16;
+            const int t0 = tl.tile(v) * 64;
+            const bool sees = t0 <= pw1 && (a.window == 0 || t0 + 63 > pw0 - a.window || t0 < a.sinks);
+            f32x16 x[2];
+            if (sees) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    x[b] = f32x16{};
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d)
+                        x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            *reinterpret_cast<const f16x8*>(kb + (2 * d * 64 + 32 * b) * 16), qf[d], x[b], 0, 0, 0);
+                }
+            }
+            const f32x4 ks4 = *reinterpret_cast<const f32x4*>(s_scale[half][0]);
+            const f32x4 vs4 = *reinterpret_cast<const f32x4*>(s_scale[half][1]);
+            if (v + 1 < v1) put(half ^ 1);
+            if (v + 2 < v1) request();
+            if (v + 3 < v1) find(v + 3);
+            if (sees) {
+                const float ksv[4] = {ks4[0], ks4[1], ks4[2], ks4[3]};
+                float vsv[4] = {vs4[0], vs4[1], vs4[2], vs4[3]};
+                // Token of score (b, e): t0 + 32 b + 8 (e / 4) + 4 g + e % 4, of sub-block 2 b + e / 8. A sub-block's
+                // factor is kept above 0 so that -inf stays -inf.
+                float sc[2][16], f[4];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[b][e] = x[b][e];
+                bool whole = t0 + 63 <= pw0 && t0 + 64 <= s.len &&
+                             (a.window == 0 || t0 > pw1 - a.window || t0 + 64 <= a.sinks);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    f[b] = fmaxf(ksv[b] * a.scale * unscale, 0x1p-126f);
+                    whole = whole && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ksv[b])) >= 0;
+                }
+                float un;
+                if (whole) {
+                    un = fmaxf(fmaxf(vsv[0], vsv[1]), fmaxf(vsv[2], vsv[3]));
+                } else {
+                    un = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        bool some = false;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int j = t0 + 16 * b + 8 * (e >> 2) + 4 * g + (e & 3);
+                            const bool seen = (ksv[b] >= 0.0f) & (j <= p) & (j < s.len) &
+                                              ((a.window == 0) | (j > p - a.window) | (j < a.sinks));
+                            sc[b >> 1][8 * (b & 1) + e] = seen ? sc[b >> 1][8 * (b & 1) + e] : kNegInf;
+                            some |= seen;
+                        }
+                        vsv[b] = some ? vsv[b] : 0.0f;  // vsv / u stays finite
+                        un = fmaxf(un, vsv[b]);
+                    }
+                    un = fmaxf(un, __shfl_xor(un, 32, kWave));
+                }
+                float mx = kNegInf;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float top = sc[b >> 1][8 * (b & 1)];
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[b >> 1][8 * (b & 1) + e]);
+                    mx = fmaxf(mx, top * f[b]);
+                }
+                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+                if (__any(mx > m + kLazy || un > u)) {
+                    const float to = mx > m + kLazy ? mx : m;
+                    const float down = decay(m, to);
+                    const float next = __builtin_amdgcn_rcpf(fmaxf(un, u));
+                    const float fade = un > u ? down * (u * next) : down;
+                    l *= down;
+#pragma unroll
+                    for (int b = 0; b < D / 32; ++b) acc[b] *= fade;
+                    m = to;
+                    inv_u = un > u ? next : inv_u;
+                    u = fmaxf(u, un);
+                }
+                const float base = m == kNegInf ? 0.0f : m;
+                f16x8 pb[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float fv = vsv[b] * inv_u;
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f[b], -base));
+                        l += w[e];
+                        w[e] *= fv;
+                    }
+                    pb[b] = __builtin_bit_cast(f16x8, pack8<f16>(w));
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            *reinterpret_cast<const f16x8*>(vb + (2 * b * D + 32 * d) * 16), pb[b], acc[d], 0, 0, 0);
+            }
+            __syncthreads();
+        }
+        l += __shfl_xor(l, 32, kWave);
+        if (real) {
+            const float inv = l == 0.0f ? 0.0f : u / l;
+            const size_t all = static_cast<size_t>(a.total) * a.hq, slot = blockIdx.z * all + row;
+            // acc[b][4 n + e] is position 32 b + 8 n + 4 g + e: i = 2 (b % 2) + n / 2, kg = 2 (n % 2) + g.
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    float o[16];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[4 * j + e] = acc[2 * c + (j >> 1)][4 * (2 * (j & 1) + n) + e] * inv;
+                    const int d = 64 * c + 16 * (2 * n + g);
+                    if (sl.count > 1) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<f32x4*>(a.part + slot * D + d + 4 * j) =
+                                f32x4{o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]};
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = o[8 * j + e];
+                            st16(out + row * D + d + 8 * j, pack8<T>(y));
+                        }
+                    }
+                }
+            if (sl.count > 1 && g == 0) {
+                float* ml = a.part + a.splits * all * D + slot * 2;
+                ml[0] = m;
+                ml[1] = l;
+            }
+        }
+    }
+}
+
 // Joins the slices of a row: out = sum_s l_s 2^(m_s - M) o_s / sum_s l_s 2^(m_s - M),
 // added in slice order. A wave per row; rows of one slice are done already.
 // Grid: rows of a sequence (strided over), batch.
@@ -410,9 +644,9 @@ __global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv
     const size_t all = static_cast<size_t>(a.total) * a.hq;
     for (int rr = blockIdx.x; rr < s.rows.count * a.hq; rr += gridDim.x) {
         const int i = rr / a.hq, hh = rr - i * a.hq;
-        const int r = i * a.group + hh % a.group, r0 = r & ~15, R = s.rows.count * a.group;
+        const int r = i * a.group + hh % a.group, r0 = r & -a.row_tile, R = s.rows.count * a.group;
         const int p0 = s.last - s.rows.count + 1 + r0 / a.group;
-        const int p1 = s.last - s.rows.count + 1 + min(r0 + 15, R - 1) / a.group;
+        const int p1 = s.last - s.rows.count + 1 + min(r0 + a.row_tile - 1, R - 1) / a.group;
         const int n = slices(a, tiles_seen(p0, p1, s.len, a.window, a.sinks).count).count;
         if (n == 1) continue;
         const size_t row = static_cast<size_t>(s.rows.first) * a.hq + rr;
@@ -437,20 +671,26 @@ __global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv
 
 // ---- host side ---------------------------------------------------------------
 
-// Slices worth having: enough blocks for kBlocksWanted, at least kTilesLeast
+// Sequences of at least kPromptFrom rows take the prompt kernel.
+constexpr int kPromptFrom = 33;
+// Slices worth having: enough blocks to fill the GPU, at least kTilesLeast
 // tiles in each.
-constexpr int kBlocksWanted = 1024, kTilesLeast = 8;
+constexpr int kTilesLeast = 8;
 struct Plan {
-    int row_tiles, splits, chunk;
+    bool prompt;
+    int row_tile, row_tiles, splits, chunk;
 };
 Plan plan(int hkv, int group, int batch, int max_q, int max_kv) {
     Plan p;
-    p.row_tiles = static_cast<int>((static_cast<long long>(max_q) * group + 15) / 16);
+    const long long rows = static_cast<long long>(max_q) * group;
+    p.prompt = rows >= kPromptFrom;
+    p.row_tile = p.prompt ? kPromptRows : 16;
+    p.row_tiles = static_cast<int>((rows + p.row_tile - 1) / p.row_tile);
     const int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
     const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
-    const long long want = (kBlocksWanted + blocks - 1) / blocks;
+    const long long want = ((p.prompt ? 512 : 1024) + blocks - 1) / blocks;
     const int most = std::max(tiles / kTilesLeast, 1);
-    p.splits = static_cast<int>(std::min<long long>(want, most));
+    p.splits = static_cast<int>(std::min<long long>(std::min<long long>(want, most), 65535));
     p.chunk = (tiles + p.splits - 1) / p.splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
     return p;
@@ -463,7 +703,10 @@ void launch_attention(const Plan& p, int batch, uint16_t* out, const uint16_t* q
                       int max_q) {
     constexpr int NB = D <= 128 ? 4 : 2;
     const int y = std::min(p.row_tiles, std::max(1, 65535 / kv.hkv)) * kv.hkv;
-    kv_decode_kernel<T, D, NB><<<dim3(p.splits, y, batch), dim3(kDecodeWaves * kWave), 0, stream()>>>(out, q, kv, a);
+    if (p.prompt)
+        kv_prompt_kernel<T, D><<<dim3(y, batch, p.splits), dim3(kPromptWaves * kWave), 0, stream()>>>(out, q, kv, a);
+    else
+        kv_decode_kernel<T, D, NB><<<dim3(p.splits, y, batch), dim3(kDecodeWaves * kWave), 0, stream()>>>(out, q, kv, a);
     if (p.splits > 1) {
         const long long rows = static_cast<long long>(max_q) * a.hq;
         kv_join_kernel<T, D><<<dim3(static_cast<unsigned>(std::min<long long>(rows, 1 << 20)), batch), dim3(kWave), 0,
@@ -488,7 +731,7 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
     max_q = std::min(max_q, total);
     AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
                total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,
-               1, 1, static_cast<float*>(workspace)};
+               16, 1, 1, static_cast<float*>(workspace)};
     Plan p = plan(cache->num_kv_heads, a.group, batch, max_q, max_kv);
     const size_t rows = static_cast<size_t>(total) * hq;
     const size_t room = workspace == nullptr ? 0 : workspace_bytes / slice_bytes(rows, cache->head_dim);
@@ -497,6 +740,7 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
         p.splits = std::max<int>(static_cast<int>(room), 1);
         p.chunk = (tiles + p.splits - 1) / p.splits;
     }
+    a.row_tile = p.row_tile;
     a.splits = p.splits;
     a.chunk = p.chunk;
     const KvView kv = kv_view(*cache);
