@@ -101,30 +101,37 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, const KvView& kv, int
     return s;
 }
 
-// A 16-token sub-block of a head: byte offset of its codes, index of its scales,
-// and whether there is such a page (if not, both name the first one, whose
-// memory is there to be read).
+// A 16-token sub-block of a head (of a sequence that has tokens): byte offset of
+// its codes, index of its scales, and whether there is such a page (if not, both
+// name the first one, whose memory is there to be read).
 struct Sub {
     size_t codes, scale;
     bool there;
 };
 __device__ __forceinline__ Sub sub_block(const KvView& kv, const Seq& s, int h, int token, int D) {
-    int page = token < s.len ? load_uniform(s.table + (token >> kv.ps_log2)) : -1;
-    const bool there = page >= 0 && page < kv.num_pages;
+    int page = load_uniform(s.table + (min(token, s.len - 1) >> kv.ps_log2));
+    const bool there = (token < s.len) & (page >= 0) & (page < kv.num_pages);
     page = there ? page : 0;
     const size_t ph = static_cast<size_t>(page) * kv.hkv + h;
     return {((ph << kv.ps_log2) + (token & ((1 << kv.ps_log2) - 1))) * D, ph, there};
 }
 
-// Maximum and sum over the four lanes that hold a column of a 16 x 16 tile.
-__device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, kWave));
-    return fmaxf(v, __shfl_xor(v, 32, kWave));
+// Values of the lane 32 away, and of the lanes 16, 32 and 48 away (those that
+// hold a column of a 32 x 32 and of a 16 x 16 tile), joined with the lane's own.
+template <typename F>
+__device__ __forceinline__ float with_half(float v, F&& join) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return join(as_float(r[0]), as_float(r[1]));
 }
-__device__ __forceinline__ float col_sum(float v) {
-    v += __shfl_xor(v, 16, kWave);
-    return v + __shfl_xor(v, 32, kWave);
+template <typename F>
+__device__ __forceinline__ float with_rows(float v, F&& join) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return with_half(join(as_float(r[0]), as_float(r[1])), join);
 }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
 
 // 2^(m - to) where to >= m may be -inf (nothing seen yet on either side).
 __device__ __forceinline__ float decay(float m, float to) {
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
                     vs[t] = some ? vs[t] : 0.0f;
                     un = fmaxf(un, vs[t]);
                 }
-                un = col_max(un);
+                un = with_rows(un, larger);
             }
             un = fmaxf(un, u);
             float mx = m;
@@ -291,7 +298,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             for (int t = 0; t < NB; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
-            mx = col_max(mx);
+            mx = with_rows(mx, larger);
             const float base = mx == kNegInf ? 0.0f : mx;
             const float down = decay(m, mx);
             l *= down;
@@ -333,7 +340,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 #pragma unroll
             for (int t = 0; t < NB; ++t) sub[t] = nsub[t];
         }
-        l = col_sum(l);
+        l = with_rows(l, plus);
         // Join the waves: lane (column, kg) of each holds d = 64 c + 16 kg + 4 j + e.
         if (kg == 0) {
             s_m[wave][col] = m;
@@ -395,7 +402,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
     }
 }
 
-// Many queries to a sequence: bound by the matrix cores and the exponentials. A
+// Many queries to a sequence: bound by the matrix cores and the VALU, which
+// takes about 1.3 times as long for the conversions and the exponentials. A
 // block of four waves takes 128 rows, 32 a wave (32 x 32 x 16 MFMAs), and goes
 // through tiles of 64 tokens. A tile's codes become fp16 once a block, on their
 // way into LDS: while a tile is multiplied, the next one's codes, which arrived
@@ -405,8 +413,17 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 //   a piece being the 8 tokens that lane half g of an MFMA's second operand
 //   holds, quads g and 2 + g. d = 64 c + 16 kg + 4 i + r stands at position
 //   64 c + 16 i + 4 kg + r, so that a wave's writes of one i are contiguous.
-// A row's maximum is raised only when a score passes it by 2^8 (weights up to
-// 2^8 then, exact all the same), so most tiles rescale nothing.
+// Every MFMA of a wave has VALU work of its own beside it, in four phases:
+//   scores of tokens 0-31     | K of the next tile converted
+//   scores of tokens 32-63    | weights of tokens 0-31
+//   V P of tokens 0-31        | weights of tokens 32-63
+//   V P of tokens 32-63       | V of the next tile converted
+// (left to the two waves of a SIMD to overlap, they did not: the waves fall
+// into step, and MFMAs and VALU took 37% and 60% of the time one after the
+// other.) A row's maximum is raised only when a score passes it by 2^8 (weights
+// up to 2^8 then, exact all the same), so most tiles rescale nothing. v_s / u
+// goes into the exponent, 2^(x - m + log2(v_s / u)), and out of it again for
+// the sum, once for a sub-block.
 // Grid: row tiles x key/value heads (the last rows, which see most, first; a
 // head's blocks next to each other in the same L2 where 8 divides the heads),
 // batch, slices.
@@ -417,9 +434,10 @@ template <typename T, int D>
 __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_prompt_kernel(uint16_t* out,
                                                                                           const uint16_t* q, KvView kv,
                                                                                           AttnArgs a) {
-    constexpr int C = D / 64, kHalf = 64 * D * 2;  // bytes of a tile of K
+    constexpr int C = D / 64, N = D / 16;  // MFMAs of a phase, dwords of K or V that a lane brings
+    constexpr int kHalf = 64 * D * 2;       // bytes of a tile of K
     __shared__ __align__(1024) uint8_t lds[2][2 * kHalf];
-    __shared__ __align__(16) float s_scale[2][2][4];  // of the sub-blocks: K's (< 0: no page), V's
+    __shared__ __align__(16) float s_scale[2][2][32][4];  // of the sub-blocks: K's (< 0: no page), log2 of V's
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 31, g = lane >> 5;
@@ -428,7 +446,7 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
     const int R = s.rows.count * a.group, tiles = (R + kPromptRows - 1) / kPromptRows;
     const int first = s.last - s.rows.count + 1;  // position of the first query
     const int kput = ((2 * (lane >> 4)) * 64 + kSub * wave + (lane & 15)) * 16;
-    const int vput = ((2 * wave + ((lane >> 2) & 1)) * D + 4 * (lane >> 4) + (lane & 3)) * 16 + ((lane >> 3) & 1) * 8;
+    const int vput = kHalf + ((2 * wave + ((lane >> 2) & 1)) * D + 4 * (lane >> 4) + (lane & 3)) * 16 + ((lane >> 3) & 1) * 8;
     for (int rt = tiles - 1 - static_cast<int>(blockIdx.x) / kv.hkv; rt >= 0; rt -= static_cast<int>(gridDim.x) / kv.hkv) {
         const int r0 = rt * kPromptRows;
         const int p0 = first + r0 / a.group, p1 = first + min(r0 + kPromptRows - 1, R - 1) / a.group;
@@ -448,155 +466,216 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
         u32x4 kr[C], vr[C];
         float ks = -1.0f, vs = 0.0f;
         Sub sub;
-        const auto find = [&](int v) { sub = sub_block(kv, s, h, tl.tile(v) * 64 + kSub * wave, D); };
-        const auto request = [&] {  // the sub-block in `sub`
+        const auto find = [&](int v) { sub = sub_block(kv, s, h, tl.tile(min(v, v1 - 1)) * 64 + kSub * wave, D); };
+        const auto request_k = [&] {  // of the sub-block in `sub`, and its scales
 #pragma unroll
             for (int c = 0; c < C; ++c) kr[c] = ld16(kv.kc + sub.codes + 1024 * c + 16 * lane);
+            ks = load_uniform(kv.ks + sub.scale);
+            vs = load_uniform(kv.vs + sub.scale);
+            ks = sub.there ? ks : -1.0f;
+            vs = sub.there ? vs : 0.0f;
+        };
+        const auto request_v = [&] {
 #pragma unroll
             for (int c = 0; c < C; ++c) vr[c] = ld16(kv.vc + sub.codes + 1024 * c + 16 * lane);
-            ks = sub.there ? load_uniform(kv.ks + sub.scale) : -1.0f;
-            vs = sub.there ? load_uniform(kv.vs + sub.scale) : 0.0f;
         };
-        const auto put = [&](int half) {  // what was requested, as fp16
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                uint8_t* k = lds[half] + kput + 8 * c * 1024;
-                *reinterpret_cast<f16x8*>(k) = codes8(kr[c][0], kr[c][1]);
-                *reinterpret_cast<f16x8*>(k + 1024) = codes8(kr[c][2], kr[c][3]);
-                uint8_t* v = lds[half] + kHalf + vput + c * 1024;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t b = vr[c][j] ^ 0x80808080u;
-                    *reinterpret_cast<u32x2*>(v + 256 * j) = u32x2{codes2<0x04010400u>(b), codes2<0x04030402u>(b)};
-                }
-            }
-            if (lane == 0) {
-                s_scale[half][0][wave] = ks;
-                s_scale[half][1][wave] = vs;
-            }
+        // Dword d of what was requested, as fp16 into LDS (after a slice's last tile once more, for nobody).
+        u32x2 before;
+        const auto put_k = [&](int half, int d) {
+            const uint32_t w = kr[d >> 2][d & 3] ^ 0x80808080u;
+            const u32x2 y = {codes2<0x04010400u>(w), codes2<0x04030402u>(w)};
+            if (d & 1)
+                *reinterpret_cast<u32x4*>(lds[half] + kput + (d >> 2) * 8192 + ((d >> 1) & 1) * 1024) =
+                    u32x4{before[0], before[1], y[0], y[1]};
+            before = y;
+        };
+        const auto put_v = [&](int half, int d) {
+            const uint32_t w = vr[d >> 2][d & 3] ^ 0x80808080u;
+            *reinterpret_cast<u32x2*>(lds[half] + vput + (d >> 2) * 1024 + (d & 3) * 256) =
+                u32x2{codes2<0x04010400u>(w), codes2<0x04030402u>(w)};
+        };
+        const auto put_scales = [&](int half) {
+            s_scale[half][g][col][wave] = g == 0 ? ks : __builtin_amdgcn_logf(vs);
         };
 
-        float m = kNegInf, l = 0.0f, u = kLeastUnit, inv_u = 0x1p126f;
+        float m = kNegInf, l = 0.0f, lu = -126.0f;  // lu: log2 u
         f32x16 acc[D / 32];
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) acc[b] = f32x16{};
         if (v0 < v1) {
             find(v0);
-            request();
-            put(0);
-            if (v0 + 1 < v1) {
-                find(v0 + 1);
-                request();
-            }
-            if (v0 + 2 < v1) find(v0 + 2);
+            request_k();
+            request_v();
+#pragma unroll
+            for (int d = 0; d < N; ++d) put_k(0, d), put_v(0, d);
+            put_scales(0);
+            find(v0 + 1);
+            request_k();
+            request_v();
+            find(v0 + 2);
         }
         __syncthreads();
         for (int v = v0; v < v1; ++v) {
             const int half = (v - v0) & 1;
-            const uint8_t *kb = lds[half] + (g * 64 + col) * 16, *vb = lds[half] + kHalf + (g * D + col) * 16;
             const int t0 = tl.tile(v) * 64;
-            const bool sees = t0 <= pw1 && (a.window == 0 || t0 + 63 > pw0 - a.window || t0 < a.sinks);
-            f32x16 x[2];
-            if (sees) {
+            // First operands of the tile's 4 N MFMAs in order, read three ahead.
+            const uint8_t *kb = lds[half] + (g * 64 + col) * 16, *vb = lds[half] + kHalf + (g * D + col) * 16;
+            f16x8 ring[4];
+            const auto read = [&](int j) {
+                if (j >= 4 * N) return;
+                const int b = j / N % 2, d = j % N;
+                const uint8_t* at = j < 2 * N ? kb + (2 * d * 64 + 32 * b) * 16
+                                              : vb + (2 * (2 * b + d / (D / 32)) * D + 32 * (d % (D / 32))) * 16;
+                ring[j & 3] = *reinterpret_cast<const f16x8*>(at);
+            };
+            read(0), read(1), read(2);
+            const f32x4 ks4 = *reinterpret_cast<const f32x4*>(s_scale[half][0][col]);
+            const f32x4 lv4 = *reinterpret_cast<const f32x4*>(s_scale[half][1][col]);
+            put_scales(half ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 x = f32x16{}, y = f32x16{};
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    x[b] = f32x16{};
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d)
-                        x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                            *reinterpret_cast<const f16x8*>(kb + (2 * d * 64 + 32 * b) * 16), qf[d], x[b], 0, 0, 0);
-                }
+            for (int d = 0; d < N; ++d) {
+                read(d + 3);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[d & 3], qf[d], x, 0, 0, 0);
+                put_k(half ^ 1, d);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const f32x4 ks4 = *reinterpret_cast<const f32x4*>(s_scale[half][0]);
-            const f32x4 vs4 = *reinterpret_cast<const f32x4*>(s_scale[half][1]);
-            if (v + 1 < v1) put(half ^ 1);
-            if (v + 2 < v1) request();
-            if (v + 3 < v1) find(v + 3);
-            if (sees) {
-                const float ksv[4] = {ks4[0], ks4[1], ks4[2], ks4[3]};
-                float vsv[4] = {vs4[0], vs4[1], vs4[2], vs4[3]};
-                // Token of score (b, e): t0 + 32 b + 8 (e / 4) + 4 g + e % 4, of sub-block 2 b + e / 8. A sub-block's
-                // factor is kept above 0 so that -inf stays -inf.
-                float sc[2][16], f[4];
+            request_k();
+            bool whole = t0 + 63 <= pw0 && t0 + 64 <= s.len && (a.window == 0 || t0 > pw1 - a.window || t0 + 64 <= a.sinks);
+            const float ksv[4] = {ks4[0], ks4[1], ks4[2], ks4[3]};
+            float lv[4] = {lv4[0], lv4[1], lv4[2], lv4[3]}, f[4];
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 4; ++b) {
+                // A sub-block's factor is kept above 0 so that -inf stays -inf.
+                f[b] = fmaxf(ksv[b] * a.scale * unscale, 0x1p-126f);
+                whole = whole && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ksv[b])) >= 0;
+            }
+            // Token of score e of half b: t0 + 32 b + 8 (e / 4) + 4 g + e % 4, of sub-block 2 b + e / 8. Scores that the
+            // row does not see become -inf; whether its maximum or u have to grow for the others.
+            float mx, lx;
+            const auto look = [&](int b, const f32x16& x, float (&sc)[16]) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[b][e] = x[b][e];
-                bool whole = t0 + 63 <= pw0 && t0 + 64 <= s.len &&
-                             (a.window == 0 || t0 > pw1 - a.window || t0 + 64 <= a.sinks);
+                for (int e = 0; e < 16; ++e) sc[e] = x[e];
+                if (!whole) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    f[b] = fmaxf(ksv[b] * a.scale * unscale, 0x1p-126f);
-                    whole = whole && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ksv[b])) >= 0;
-                }
-                float un;
-                if (whole) {
-                    un = fmaxf(fmaxf(vsv[0], vsv[1]), fmaxf(vsv[2], vsv[3]));
-                } else {
-                    un = 0.0f;
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
+                    for (int n = 0; n < 2; ++n) {
                         bool some = false;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int j = t0 + 16 * b + 8 * (e >> 2) + 4 * g + (e & 3);
-                            const bool seen = (ksv[b] >= 0.0f) & (j <= p) & (j < s.len) &
+                        for (int e = 8 * n; e < 8 * n + 8; ++e) {
+                            const int j = t0 + 32 * b + 8 * (e >> 2) + 4 * g + (e & 3);
+                            const bool seen = (ksv[2 * b + n] >= 0.0f) & (j <= p) & (j < s.len) &
                                               ((a.window == 0) | (j > p - a.window) | (j < a.sinks));
-                            sc[b >> 1][8 * (b & 1) + e] = seen ? sc[b >> 1][8 * (b & 1) + e] : kNegInf;
+                            sc[e] = seen ? sc[e] : kNegInf;
                             some |= seen;
                         }
-                        vsv[b] = some ? vsv[b] : 0.0f;  // vsv / u stays finite
-                        un = fmaxf(un, vsv[b]);
+                        lv[2 * b + n] = some ? lv[2 * b + n] : kNegInf;
                     }
-                    un = fmaxf(un, __shfl_xor(un, 32, kWave));
                 }
-                float mx = kNegInf;
+                float top[2];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    float top = sc[b >> 1][8 * (b & 1)];
+                for (int n = 0; n < 2; ++n) {
+                    top[n] = sc[8 * n];
 #pragma unroll
-                    for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[b >> 1][8 * (b & 1) + e]);
-                    mx = fmaxf(mx, top * f[b]);
+                    for (int e = 1; e < 8; ++e) top[n] = fmaxf(top[n], sc[8 * n + e]);
+                    top[n] *= f[2 * b + n];
                 }
-                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                if (__any(mx > m + kLazy || un > u)) {
-                    const float to = mx > m + kLazy ? mx : m;
-                    const float down = decay(m, to);
-                    const float next = __builtin_amdgcn_rcpf(fmaxf(un, u));
-                    const float fade = un > u ? down * (u * next) : down;
-                    l *= down;
+                mx = with_half(fmaxf(top[0], top[1]), larger);
+                lx = fmaxf(lv[2 * b], lv[2 * b + 1]);
+                if (!whole) lx = with_half(lx, larger);
+                return __any((mx > m + kLazy) | (lx > lu));
+            };
+            const auto rescale = [&] {
+                const float to = mx > m + kLazy ? mx : m;
+                const float down = decay(m, to);
+                const float fade = down * __builtin_amdgcn_exp2f(fminf(lu - lx, 0.0f));
+                l *= down;
 #pragma unroll
-                    for (int b = 0; b < D / 32; ++b) acc[b] *= fade;
-                    m = to;
-                    inv_u = un > u ? next : inv_u;
-                    u = fmaxf(u, un);
-                }
+                for (int b = 0; b < D / 32; ++b) acc[b] *= fade;
+                m = to;
+                lu = fmaxf(lu, lx);
+            };
+            // Weights of the scores [16 d / N, 16 (d + 1) / N) of half b; log2(v_s / u) is kept where its inverse is
+            // finite: below, V's part is nothing beside what u stands for.
+            float off[2], back[2], w[16];
+            const auto begin = [&](int b) {
                 const float base = m == kNegInf ? 0.0f : m;
-                f16x8 pb[4];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const float fv = vsv[b] * inv_u;
-                    float w[8];
+                for (int n = 0; n < 2; ++n) {
+                    const float d = fmaxf(lv[2 * b + n] - lu, -60.0f);
+                    off[n] = d - base;
+                    back[n] = __builtin_amdgcn_exp2f(-d);
+                }
+            };
+            const auto weigh = [&](int b, int d, const float (&sc)[16], uint32_t (&pk)[8]) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f[b], -base));
-                        l += w[e];
-                        w[e] *= fv;
+                for (int e = 16 * d / N; e < 16 * (d + 1) / N; ++e) {
+                    const int n = e >> 3;
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], f[2 * b + n], off[n]));
+                    if (e & 1) {
+                        pk[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{w[e - 1], w[e]}, f16x2));
+                        w[e] += w[e - 1];
+                        if ((e & 7) != 1) w[e] += w[e - 2];
+                        if ((e & 7) == 7) l = __builtin_fmaf(w[e], back[n], l);
                     }
-                    pb[b] = __builtin_bit_cast(f16x8, pack8<f16>(w));
+                }
+            };
+            float sc[16], sd[16];
+            uint32_t pa[8], pb[8];
+            const auto operand = [](const uint32_t (&pk)[8], int n) {
+                return __builtin_bit_cast(f16x8, u32x4{pk[4 * n], pk[4 * n + 1], pk[4 * n + 2], pk[4 * n + 3]});
+            };
+            const auto add = [&](int d, int j, const uint32_t (&pk)[8]) {
+                acc[d % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j & 3], operand(pk, d / (D / 32)),
+                                                                           acc[d % (D / 32)], 0, 0, 0);
+            };
+            if (look(0, x, sc)) rescale();
+            begin(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < N; ++d) {
+                read(N + d + 3);
+                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[(N + d) & 3], qf[d], y, 0, 0, 0);
+                weigh(0, d, sc, pa);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) __asm__ volatile("" : "+v"(pa[k]));  // weighed here, not where it is used
+            if (look(1, y, sd)) {
+                // What is weighed already counts under the old maximum and u.
+#pragma unroll
+                for (int d = 0; d < N; ++d) {
+                    const f16x8 first = *reinterpret_cast<const f16x8*>(vb + (2 * (d / (D / 32)) * D + 32 * (d % (D / 32))) * 16);
+                    acc[d % (D / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(first, operand(pa, d / (D / 32)),
+                                                                               acc[d % (D / 32)], 0, 0, 0);
                 }
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                            *reinterpret_cast<const f16x8*>(vb + (2 * b * D + 32 * d) * 16), pb[b], acc[d], 0, 0, 0);
+                for (int k = 0; k < 8; ++k) pa[k] = 0;
+                rescale();
             }
+            begin(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < N; ++d) {
+                read(2 * N + d + 3);
+                add(d, 2 * N + d, pa);
+                weigh(1, d, sd, pb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int d = 0; d < N; ++d) {
+                read(3 * N + d + 3);
+                add(d, 3 * N + d, pb);
+                put_v(half ^ 1, d);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            request_v();
+            find(v + 3);
             __syncthreads();
         }
-        l += __shfl_xor(l, 32, kWave);
+        l = with_half(l, plus);
         if (real) {
-            const float inv = l == 0.0f ? 0.0f : u / l;
+            const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(lu) / l;
             const size_t all = static_cast<size_t>(a.total) * a.hq, slot = blockIdx.z * all + row;
             // acc[b][4 n + e] is position 32 b + 8 n + 4 g + e: i = 2 (b % 2) + n / 2, kg = 2 (n % 2) + g.
 #pragma unroll
@@ -633,14 +712,20 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
     }
 }
 
-// Joins the slices of a row: out = sum_s l_s 2^(m_s - M) o_s / sum_s l_s 2^(m_s - M),
-// added in slice order. A wave per row; rows of one slice are done already.
+// Joins the slices of a row: out = sum_s l_s 2^(m_s - M) o_s / sum_s l_s 2^(m_s - M).
+// Four waves a row, wave w the slices w, w + 4, ..., several on their way at a
+// time (one wave and one slice at a time took 37 us for 32 rows of 128 slices,
+// longer than the attention itself). Rows of one slice are done already.
 // Grid: rows of a sequence (strided over), batch.
+constexpr int kJoinWaves = 4;
+
 template <typename T, int D>
-__global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv, AttnArgs a) {
+__global__ __launch_bounds__(kJoinWaves * kWave) void kv_join_kernel(uint16_t* out, KvView kv, AttnArgs a) {
     constexpr int C = D / 64;
+    __shared__ float s_o[kJoinWaves][D], s_l[kJoinWaves];
     const Seq s = sequence(a, kv, blockIdx.y);
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const size_t all = static_cast<size_t>(a.total) * a.hq;
     for (int rr = blockIdx.x; rr < s.rows.count * a.hq; rr += gridDim.x) {
         const int i = rr / a.hq, hh = rr - i * a.hq;
@@ -651,21 +736,54 @@ __global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv
         if (n == 1) continue;
         const size_t row = static_cast<size_t>(s.rows.first) * a.hq + rr;
         const float* ml = a.part + a.splits * all * D + row * 2;
+        const float* po = a.part + row * D + lane;
         float M = kNegInf;
         for (int x = lane; x < n; x += kWave) M = fmaxf(M, ml[x * all * 2]);
         M = wave_max_f32(M);
         float L = 0.0f, o[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) o[c] = 0.0f;
-        for (int x = 0; x < n; ++x) {
-            const float w = ml[x * all * 2 + 1] * decay(ml[x * all * 2], M);
-            L += w;
-#pragma unroll
-            for (int c = 0; c < C; ++c) o[c] += w * a.part[(x * all + row) * D + 64 * c + lane];
+        for (int x0 = wave * kWave; x0 < n; x0 += kJoinWaves * kWave) {
+            // 64 slices' weights, one to a lane.
+            const int mine = x0 + lane;
+            const float w = mine < n ? ml[mine * all * 2 + 1] * decay(ml[mine * all * 2], M) : 0.0f;
+            L += wave_sum_f32(w);
         }
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        for (int x0 = 0; x0 < n; x0 += kWave) {
+            const int mine = x0 + lane, end = min(n - x0, kWave);
+            const float w = mine < n ? ml[mine * all * 2 + 1] * decay(ml[mine * all * 2], M) : 0.0f;
+            for (int x = wave; x < end; x += 8 * kJoinWaves) {
+                float v[8][C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) out[row * D + 64 * c + lane] = from_f32<T>(o[c] * inv);
+                for (int k = 0; k < 8; ++k) {
+                    const int y = min(x + k * kJoinWaves, end - 1);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) v[k][c] = po[(x0 + y) * all * D + 64 * c];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int y = x + k * kJoinWaves;
+                    const float f = y < end ? __shfl(w, y, kWave) : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) o[c] += f * v[k][c];
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) s_o[wave][64 * c + lane] = o[c];
+        if (lane == 0) s_l[wave] = L;
+        __syncthreads();
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w) L += s_l[w];
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        for (int d = threadIdx.x; d < D; d += kJoinWaves * kWave) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kJoinWaves; ++w) v += s_o[w][d];
+            out[row * D + d] = from_f32<T>(v * inv);
+        }
+        __syncthreads();
     }
 }
 
@@ -673,9 +791,12 @@ __global__ __launch_bounds__(kWave) void kv_join_kernel(uint16_t* out, KvView kv
 
 // Sequences of at least kPromptFrom rows take the prompt kernel.
 constexpr int kPromptFrom = 33;
-// Slices worth having: enough blocks to fill the GPU, at least kTilesLeast
-// tiles in each.
-constexpr int kTilesLeast = 8;
+// Slices worth having: two blocks to a CU (that many are resident; 64 sequences
+// of up to 4096 tokens: 67 us with 512 blocks in one slice, 75-80 us with 1024
+// in two, and the join), a tile to a wave at least. Below 1024 tokens the join
+// costs more than it saves (500 tokens: 7.4 us in one slice, 9.7 in two; 4096
+// tokens of one sequence: 13.7 us in 16 slices, 15.3 in 8).
+constexpr int kBlocksWanted = 512, kTilesLeast = 4;
 struct Plan {
     bool prompt;
     int row_tile, row_tiles, splits, chunk;
@@ -688,8 +809,8 @@ Plan plan(int hkv, int group, int batch, int max_q, int max_kv) {
     p.row_tiles = static_cast<int>((rows + p.row_tile - 1) / p.row_tile);
     const int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
     const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
-    const long long want = ((p.prompt ? 512 : 1024) + blocks - 1) / blocks;
-    const int most = std::max(tiles / kTilesLeast, 1);
+    const long long want = (kBlocksWanted + blocks - 1) / blocks;
+    const int most = tiles < 4 * kTilesLeast ? 1 : tiles / kTilesLeast;
     p.splits = static_cast<int>(std::min<long long>(std::min<long long>(want, most), 65535));
     p.chunk = (tiles + p.splits - 1) / p.splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
@@ -709,8 +830,8 @@ void launch_attention(const Plan& p, int batch, uint16_t* out, const uint16_t* q
         kv_decode_kernel<T, D, NB><<<dim3(p.splits, y, batch), dim3(kDecodeWaves * kWave), 0, stream()>>>(out, q, kv, a);
     if (p.splits > 1) {
         const long long rows = static_cast<long long>(max_q) * a.hq;
-        kv_join_kernel<T, D><<<dim3(static_cast<unsigned>(std::min<long long>(rows, 1 << 20)), batch), dim3(kWave), 0,
-                               stream()>>>(out, kv, a);
+        kv_join_kernel<T, D><<<dim3(static_cast<unsigned>(std::min<long long>(rows, 1 << 20)), batch),
+                               dim3(kJoinWaves * kWave), 0, stream()>>>(out, kv, a);
     }
 }
 
