@@ -46,18 +46,25 @@ struct AttnArgs {
     float* part;        // their outputs [splits][total hq][D], then (m, l) [splits][total hq]
 };
 
-// Two int8 codes (bytes SEL0 and SEL1 of one dword) as exact fp16 values: biased
-// to u = q + 128, placed under an fp16 exponent of 2^10, 1152 subtracted.
+// Two codes (two bytes of a dword, which hold code + 128) as exact fp16 values:
+// placed under an fp16 exponent of 2^10, 1152 subtracted.
 template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes2(uint32_t biased) {
+__device__ __forceinline__ uint32_t codes2(uint32_t bytes) {
     const f16x2 bias = {static_cast<f16>(-1152.0f), static_cast<f16>(-1152.0f)};
-    const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, biased, SEL)) + bias;
+    const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, bytes, SEL)) + bias;
     return __builtin_bit_cast(uint32_t, v);
 }
 __device__ __forceinline__ f16x8 codes8(uint32_t lo, uint32_t hi) {
-    const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
-    return __builtin_bit_cast(f16x8, u32x4{codes2<0x04010400u>(a), codes2<0x04030402u>(a), codes2<0x04010400u>(b),
-                                           codes2<0x04030402u>(b)});
+    return __builtin_bit_cast(f16x8, u32x4{codes2<0x04010400u>(lo), codes2<0x04030402u>(lo), codes2<0x04010400u>(hi),
+                                           codes2<0x04030402u>(hi)});
+}
+
+// The larger of three (fmaxf would first make NaNs of either kind quiet, an
+// operation for each of its operands; here a NaN loses either way).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    __asm__("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
 }
 
 // The tokens that a run of queries (positions p0 .. p1) sees, in tiles of 64:
@@ -130,7 +137,7 @@ __device__ __forceinline__ float with_rows(float v, F&& join) {
     const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
     return with_half(join(as_float(r[0]), as_float(r[1])), join);
 }
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float larger(float a, float b) { return max3(a, b, b); }
 __device__ __forceinline__ float plus(float a, float b) { return a + b; }
 
 // 2^(m - to) where to >= m may be -inf (nothing seen yet on either side).
@@ -260,10 +267,10 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             if (more) load_k(nsub);
             // Scores; those of tokens that a row does not see become -inf.
             const int t0 = token_of(step);
-            bool whole = t0 + 16 * NB - 1 <= p0 && t0 + 16 * NB <= s.len &&
-                         (a.window == 0 || t0 > p1 - a.window || t0 + 16 * NB <= a.sinks);
+            bool whole = (t0 + 16 * NB - 1 <= p0) & (t0 + 16 * NB <= s.len) &
+                         ((a.window == 0) | (t0 > p1 - a.window) | (t0 + 16 * NB <= a.sinks));
 #pragma unroll
-            for (int t = 0; t < NB; ++t) whole = whole && sub[t].there;
+            for (int t = 0; t < NB; ++t) whole = whole & sub[t].there;
             float sc[NB][4];
 #pragma unroll
             for (int t = 0; t < NB; ++t) {
@@ -295,9 +302,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             un = fmaxf(un, u);
             float mx = m;
 #pragma unroll
-            for (int t = 0; t < NB; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
+            for (int t = 0; t < NB; ++t) mx = max3(max3(sc[t][0], sc[t][1], sc[t][2]), sc[t][3], mx);
             mx = with_rows(mx, larger);
             const float base = mx == kNegInf ? 0.0f : mx;
             const float down = decay(m, mx);
@@ -482,7 +487,7 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
         // Dword d of what was requested, as fp16 into LDS (after a slice's last tile once more, for nobody).
         u32x2 before;
         const auto put_k = [&](int half, int d) {
-            const uint32_t w = kr[d >> 2][d & 3] ^ 0x80808080u;
+            const uint32_t w = kr[d >> 2][d & 3];
             const u32x2 y = {codes2<0x04010400u>(w), codes2<0x04030402u>(w)};
             if (d & 1)
                 *reinterpret_cast<u32x4*>(lds[half] + kput + (d >> 2) * 8192 + ((d >> 1) & 1) * 1024) =
@@ -490,7 +495,7 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
             before = y;
         };
         const auto put_v = [&](int half, int d) {
-            const uint32_t w = vr[d >> 2][d & 3] ^ 0x80808080u;
+            const uint32_t w = vr[d >> 2][d & 3];
             *reinterpret_cast<u32x2*>(lds[half] + vput + (d >> 2) * 1024 + (d & 3) * 256) =
                 u32x2{codes2<0x04010400u>(w), codes2<0x04030402u>(w)};
         };
@@ -542,15 +547,17 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
                 __builtin_amdgcn_sched_barrier(0);
             }
             request_k();
-            bool whole = t0 + 63 <= pw0 && t0 + 64 <= s.len && (a.window == 0 || t0 > pw1 - a.window || t0 + 64 <= a.sinks);
+            bool whole = (t0 + 63 <= pw0) & (t0 + 64 <= s.len) &
+                         ((a.window == 0) | (t0 > pw1 - a.window) | (t0 + 64 <= a.sinks));
             const float ksv[4] = {ks4[0], ks4[1], ks4[2], ks4[3]};
             float lv[4] = {lv4[0], lv4[1], lv4[2], lv4[3]}, f[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 // A sub-block's factor is kept above 0 so that -inf stays -inf.
                 f[b] = fmaxf(ksv[b] * a.scale * unscale, 0x1p-126f);
-                whole = whole && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ksv[b])) >= 0;
             }
+            const float least = fminf(fminf(ksv[0], ksv[1]), fminf(ksv[2], ksv[3]));
+            whole = whole & (__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, least)) >= 0);
             // Token of score e of half b: t0 + 32 b + 8 (e / 4) + 4 g + e % 4, of sub-block 2 b + e / 8. Scores that the
             // row does not see become -inf; whether its maximum or u have to grow for the others.
             float mx, lx;
@@ -575,13 +582,11 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
                 float top[2];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    top[n] = sc[8 * n];
-#pragma unroll
-                    for (int e = 1; e < 8; ++e) top[n] = fmaxf(top[n], sc[8 * n + e]);
-                    top[n] *= f[2 * b + n];
+                    const float* c = sc + 8 * n;
+                    top[n] = max3(max3(c[0], c[1], c[2]), max3(c[3], c[4], c[5]), max3(c[6], c[7], c[7])) * f[2 * b + n];
                 }
-                mx = with_half(fmaxf(top[0], top[1]), larger);
-                lx = fmaxf(lv[2 * b], lv[2 * b + 1]);
+                mx = with_half(larger(top[0], top[1]), larger);
+                lx = larger(lv[2 * b], lv[2 * b + 1]);
                 if (!whole) lx = with_half(lx, larger);
                 return __any((mx > m + kLazy) | (lx > lu));
             };

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
 #pragma unroll
             for (int j = 0; j < 2; ++j) in[c][j] = is_new ? ld16_stream(row + 64 * c + 8 * j) : zero;
 #pragma unroll
-        for (int c = 0; c < C; ++c) old[c] = has_old ? ld16(mine + 1024 * c) : zero;
+        for (int c = 0; c < C; ++c) old[c] = has_old ? ld16(mine + 1024 * c) ^ kKvBias : zero;
         const float so = lo > 0 ? scales[ph] : 0.0f;
         uint32_t m = 0;
 #pragma unroll
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
                     q[i] = (o & keep) | (q[i] & ~keep);
                 }
             }
-            st16(mine + 1024 * c, q);
+            st16(mine + 1024 * c, q ^ kKvBias);
         }
     }
 }
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(512) void kv_read_kernel(KvView kv, uint16_t* k, ui
                               static_cast<size_t>(wave) * kSub * D + lane * 16;
         u32x4 q[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) q[c] = there ? ld16(mine + 1024 * c) : u32x4{0, 0, 0, 0};
+        for (int c = 0; c < C; ++c) q[c] = there ? ld16(mine + 1024 * c) ^ kKvBias : u32x4{0, 0, 0, 0};
         const float s = there ? load_uniform((is_v ? kv.vs : kv.ks) + ph) : 0.0f;
         uint16_t* row = x + static_cast<ptrdiff_t>(t0 + slot - start) * kv.hkv * D + 16 * kg;
 #pragma unroll

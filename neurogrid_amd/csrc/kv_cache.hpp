@@ -4,7 +4,8 @@
 // A page and head holds page_size x D codes as page_size / 16 sub-blocks of 16
 // tokens, each D / 64 chunks of 1 KiB: 64 pieces of 16 bytes, one per lane of
 // a wave, in the order in which a 16 x 16 x 32 MFMA takes its first operand, so
-// that attention loads whole KiB straight into registers.
+// that attention loads whole KiB straight into registers. A byte holds its code +
+// 128, which v_perm turns into fp16 with one subtraction.
 //   K: piece (kg, t) = 16 kg + t holds token t, d = 64 c + 16 kg + 0 .. 15.
 //   V: piece (kg, q, r) = 16 kg + 4 q + r holds in dword i the tokens 4 q ..
 //      4 q + 3 of d = 64 c + 16 kg + 4 i + r: K's order with each 4 x 4 block of
@@ -17,7 +18,8 @@
 
 namespace ng {
 
-constexpr int kSub = 16;  // tokens of a sub-block
+constexpr int kSub = 16;                    // tokens of a sub-block
+constexpr uint32_t kKvBias = 0x80808080u;  // codes to bytes and back
 
 // A cache as the kernels take it; ps_log2: page_size = 1 << ps_log2.
 struct KvView {

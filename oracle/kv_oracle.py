@@ -3,7 +3,7 @@
 Quantisation is restated in fp32, operation by operation (codes and scales are
 compared bit for bit); attention in 64 bits; the page table in plain loops.
 Codes are kept as [pages, heads, page_size, D] in token order; pack / unpack
-translate the library's order.
+translate the library's order (its bytes hold code + 128).
 """
 from __future__ import annotations
 
@@ -17,26 +17,26 @@ F = np.float32
 def unpack_k(raw: np.ndarray, D: int, page: int) -> np.ndarray:
     """Library bytes [pages, heads, page D] of K -> codes [pages, heads, page, D]."""
     P, H = raw.shape[:2]
-    v = raw.view(np.int8).reshape(P, H, page // 16, D // 64, 4, 16, 16)  # sub, chunk, kg, token, e
+    v = (raw.view(np.uint8) ^ 0x80).view(np.int8).reshape(P, H, page // 16, D // 64, 4, 16, 16)  # sub, chunk, kg, token, e
     return v.transpose(0, 1, 2, 5, 3, 4, 6).reshape(P, H, page, D).copy()
 
 
 def pack_k(codes: np.ndarray) -> np.ndarray:
     P, H, page, D = codes.shape
-    v = codes.reshape(P, H, page // 16, 16, D // 64, 4, 16)
+    v = (codes.view(np.uint8) ^ 0x80).reshape(P, H, page // 16, 16, D // 64, 4, 16)
     return v.transpose(0, 1, 2, 4, 5, 3, 6).reshape(P, H, page * D).copy()
 
 
 def unpack_v(raw: np.ndarray, D: int, page: int) -> np.ndarray:
     P, H = raw.shape[:2]
-    v = raw.view(np.int8).reshape(P, H, page // 16, D // 64, 4, 4, 4, 4, 4)  # sub, chunk, kg, q, r, i, tt
+    v = (raw.view(np.uint8) ^ 0x80).view(np.int8).reshape(P, H, page // 16, D // 64, 4, 4, 4, 4, 4)  # sub, chunk, kg, q, r, i, tt
     # token = 4 q + tt, d = 64 c + 16 kg + 4 i + r
     return v.transpose(0, 1, 2, 5, 8, 3, 4, 7, 6).reshape(P, H, page, D).copy()
 
 
 def pack_v(codes: np.ndarray) -> np.ndarray:
     P, H, page, D = codes.shape
-    v = codes.reshape(P, H, page // 16, 4, 4, D // 64, 4, 4, 4)  # sub, q, tt, chunk, kg, i, r
+    v = (codes.view(np.uint8) ^ 0x80).reshape(P, H, page // 16, 4, 4, D // 64, 4, 4, 4)  # sub, q, tt, chunk, kg, i, r
     return v.transpose(0, 1, 2, 5, 6, 3, 8, 7, 4).reshape(P, H, page * D).copy()
 
 

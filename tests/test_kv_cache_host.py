@@ -128,8 +128,8 @@ def test_packing_is_a_permutation_and_its_formula():
             t, d = int(rng.integers(page)), int(rng.integers(D))
             base = (t // 16) * 16 * D + (d // 64) * 1024
             kg, e, tt = (d % 64) // 16, d % 16, t % 16
-            assert k[1, 2, base + (16 * kg + tt) * 16 + e] == codes[1, 2, t, d]
-            assert v[1, 2, base + (16 * kg + 4 * (tt // 4) + e % 4) * 16 + 4 * (e // 4) + tt % 4] == codes[1, 2, t, d]
+            assert k[1, 2, base + (16 * kg + tt) * 16 + e] == int(codes[1, 2, t, d]) + 128
+            assert v[1, 2, base + (16 * kg + 4 * (tt // 4) + e % 4) * 16 + 4 * (e // 4) + tt % 4] == int(codes[1, 2, t, d]) + 128
 
 
 def test_append_by_hand():
