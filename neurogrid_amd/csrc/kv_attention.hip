@@ -718,27 +718,29 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
 }
 
 // Joins the slices of a row: out = sum_s l_s 2^(m_s - M) o_s / sum_s l_s 2^(m_s - M).
-// Four waves a row, wave w the slices w, w + 4, ..., several on their way at a
-// time (one wave and one slice at a time took 37 us for 32 rows of 128 slices,
-// longer than the attention itself). Rows of one slice are done already.
-// Grid: rows of a sequence (strided over), batch.
+// WAVES waves a row, wave w the slices w, w + WAVES, ..., eight on their way at a
+// time (one after the other took 37 us for 32 rows of 128 slices, longer than
+// the attention itself); a block has four waves, so 4 / WAVES rows. Rows of one
+// slice are done already. Grid: rows of a sequence (strided over), batch.
 constexpr int kJoinWaves = 4;
 
-template <typename T, int D>
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(kJoinWaves * kWave) void kv_join_kernel(uint16_t* out, KvView kv, AttnArgs a) {
-    constexpr int C = D / 64;
-    __shared__ float s_o[kJoinWaves][D], s_l[kJoinWaves];
+    constexpr int C = D / 64, kRows = kJoinWaves / WAVES;
+    __shared__ float s_o[kJoinWaves][D];
     const Seq s = sequence(a, kv, blockIdx.y);
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const size_t all = static_cast<size_t>(a.total) * a.hq;
-    for (int rr = blockIdx.x; rr < s.rows.count * a.hq; rr += gridDim.x) {
+    const int rows = s.rows.count * a.hq;
+    for (int first = blockIdx.x * kRows; first < rows; first += gridDim.x * kRows) {
+        const int rr = min(first + wave / WAVES, rows - 1);  // a block's last rows may be the same one
         const int i = rr / a.hq, hh = rr - i * a.hq;
         const int r = i * a.group + hh % a.group, r0 = r & -a.row_tile, R = s.rows.count * a.group;
         const int p0 = s.last - s.rows.count + 1 + r0 / a.group;
         const int p1 = s.last - s.rows.count + 1 + min(r0 + a.row_tile - 1, R - 1) / a.group;
         const int n = slices(a, tiles_seen(p0, p1, s.len, a.window, a.sinks).count).count;
-        if (n == 1) continue;
+        if (n == 1) continue;  // the whole block's where WAVES is 4; a wave's own otherwise, which waits for nobody
         const size_t row = static_cast<size_t>(s.rows.first) * a.hq + rr;
         const float* ml = a.part + a.splits * all * D + row * 2;
         const float* po = a.part + row * D + lane;
@@ -748,47 +750,44 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void kv_join_kernel(uint16_t* o
         float L = 0.0f, o[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) o[c] = 0.0f;
-        for (int x0 = wave * kWave; x0 < n; x0 += kJoinWaves * kWave) {
-            // 64 slices' weights, one to a lane.
-            const int mine = x0 + lane;
-            const float w = mine < n ? ml[mine * all * 2 + 1] * decay(ml[mine * all * 2], M) : 0.0f;
-            L += wave_sum_f32(w);
-        }
         for (int x0 = 0; x0 < n; x0 += kWave) {
+            // 64 slices' weights, one to a lane.
             const int mine = x0 + lane, end = min(n - x0, kWave);
             const float w = mine < n ? ml[mine * all * 2 + 1] * decay(ml[mine * all * 2], M) : 0.0f;
-            for (int x = wave; x < end; x += 8 * kJoinWaves) {
+            L += wave_sum_f32(w);
+            for (int x = wave % WAVES; x < end; x += 8 * WAVES) {
                 float v[8][C];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int y = min(x + k * kJoinWaves, end - 1);
+                    const int y = min(x + k * WAVES, end - 1);
 #pragma unroll
                     for (int c = 0; c < C; ++c) v[k][c] = po[(x0 + y) * all * D + 64 * c];
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int y = x + k * kJoinWaves;
+                    const int y = x + k * WAVES;
                     const float f = y < end ? __shfl(w, y, kWave) : 0.0f;
 #pragma unroll
                     for (int c = 0; c < C; ++c) o[c] += f * v[k][c];
                 }
             }
         }
-#pragma unroll
-        for (int c = 0; c < C; ++c) s_o[wave][64 * c + lane] = o[c];
-        if (lane == 0) s_l[wave] = L;
-        __syncthreads();
-        L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kJoinWaves; ++w) L += s_l[w];
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        for (int d = threadIdx.x; d < D; d += kJoinWaves * kWave) {
-            float v = 0.0f;
+        if constexpr (WAVES == 1) {
 #pragma unroll
-            for (int w = 0; w < kJoinWaves; ++w) v += s_o[w][d];
-            out[row * D + d] = from_f32<T>(v * inv);
+            for (int c = 0; c < C; ++c) out[row * D + 64 * c + lane] = from_f32<T>(o[c] * inv);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) s_o[wave][64 * c + lane] = o[c];
+            __syncthreads();
+            for (int d = threadIdx.x; d < D; d += kJoinWaves * kWave) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kJoinWaves; ++w) v += s_o[w][d];
+                out[row * D + d] = from_f32<T>(v * inv);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -796,17 +795,45 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void kv_join_kernel(uint16_t* o
 
 // Sequences of at least kPromptFrom rows take the prompt kernel.
 constexpr int kPromptFrom = 33;
-// Slices worth having: two blocks to a CU (that many are resident; 64 sequences
-// of up to 4096 tokens: 67 us with 512 blocks in one slice, 75-80 us with 1024
-// in two, and the join), a tile to a wave at least. Below 1024 tokens the join
-// costs more than it saves (500 tokens: 7.4 us in one slice, 9.7 in two; 4096
-// tokens of one sequence: 13.7 us in 16 slices, 15.3 in 8).
+// Slices worth having with few queries: two blocks to a CU (that many are
+// resident; 64 sequences of up to 4096 tokens: 67 us with 512 blocks in one
+// slice, 75-80 us with 1024 in two, and the join), a tile to a wave at least.
+// Below 1024 tokens the join costs more than it saves (500 tokens: 7.4 us in
+// one slice, 9.7 in two; 4096 tokens of one sequence: 13 us in 16 slices, 15 in 8).
 constexpr int kBlocksWanted = 512, kTilesLeast = 4;
 struct Plan {
     bool prompt;
     int row_tile, row_tiles, splits, chunk;
 };
-Plan plan(int hkv, int group, int batch, int max_q, int max_kv) {
+
+size_t slice_bytes(size_t rows, int D) { return rows * (D + 2) * sizeof(float); }
+
+// Slices worth having with many queries, from how long a launch would take: a
+// tile of 64 tokens at D = 128 takes a block 1.4 us where it has a CU to
+// itself and 2.4 us where two share one (as many as are resident up to D =
+// 128); the join, 5 us and its traffic at 4 TB/s. A prompt from its first
+// token on sees half its tiles on average. (512 queries behind 8000 tokens, 8
+// heads: 178 us in one slice, 122 in two, 106 in four; a prompt of 1000, 32
+// heads: 31 us in one slice, 50 in two.)
+int prompt_splits(const Plan& p, int D, long long blocks, long long rows, int max_q, int tiles) {
+    const int resident = D <= 128 ? 512 : 256;
+    const double average = std::max(tiles - max_q / 128.0, tiles * 0.5);
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= 64 && s <= std::max(tiles / kTilesLeast, 1); ++s) {
+        const int chunk = (tiles + s - 1) / s;
+        const double each = (blocks * s <= 256 ? 1.4 : D <= 128 ? 2.4 : 1.4) * D / 128;
+        double t = std::max(chunk * each, average * static_cast<double>(blocks) / resident * each);
+        if (s > 1) t += 5.0 + static_cast<double>(s) * 2.0 * static_cast<double>(slice_bytes(rows, D)) / 4e6;
+        if (s == 1 || t < least) {
+            best = s;
+            least = t;
+        }
+    }
+    return best;
+}
+
+Plan plan(int hkv, int group, int D, int batch, int max_q, int max_kv) {
     Plan p;
     const long long rows = static_cast<long long>(max_q) * group;
     p.prompt = rows >= kPromptFrom;
@@ -816,13 +843,12 @@ Plan plan(int hkv, int group, int batch, int max_q, int max_kv) {
     const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
     const long long want = (kBlocksWanted + blocks - 1) / blocks;
     const int most = tiles < 4 * kTilesLeast ? 1 : tiles / kTilesLeast;
-    p.splits = static_cast<int>(std::min<long long>(std::min<long long>(want, most), 65535));
+    p.splits = p.prompt ? prompt_splits(p, D, blocks, rows * hkv * batch, max_q, tiles)
+                        : static_cast<int>(std::min<long long>(want, most));
     p.chunk = (tiles + p.splits - 1) / p.splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
     return p;
 }
-
-size_t slice_bytes(size_t rows, int D) { return rows * (D + 2) * sizeof(float); }
 
 template <typename T, int D>
 void launch_attention(const Plan& p, int batch, uint16_t* out, const uint16_t* q, const KvView& kv, const AttnArgs& a,
@@ -835,8 +861,11 @@ void launch_attention(const Plan& p, int batch, uint16_t* out, const uint16_t* q
         kv_decode_kernel<T, D, NB><<<dim3(p.splits, y, batch), dim3(kDecodeWaves * kWave), 0, stream()>>>(out, q, kv, a);
     if (p.splits > 1) {
         const long long rows = static_cast<long long>(max_q) * a.hq;
-        kv_join_kernel<T, D><<<dim3(static_cast<unsigned>(std::min<long long>(rows, 1 << 20)), batch),
-                               dim3(kJoinWaves * kWave), 0, stream()>>>(out, kv, a);
+        const auto grid = [&](int per) { return dim3(static_cast<unsigned>(std::min<long long>((rows + per - 1) / per, 1 << 20)), batch); };
+        if (p.splits <= 8)
+            kv_join_kernel<T, D, 1><<<grid(kJoinWaves), dim3(kJoinWaves * kWave), 0, stream()>>>(out, kv, a);
+        else
+            kv_join_kernel<T, D, kJoinWaves><<<grid(1), dim3(kJoinWaves * kWave), 0, stream()>>>(out, kv, a);
     }
 }
 
@@ -858,7 +887,7 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
     AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
                total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,
                16, 1, 1, static_cast<float*>(workspace)};
-    Plan p = plan(cache->num_kv_heads, a.group, batch, max_q, max_kv);
+    Plan p = plan(cache->num_kv_heads, a.group, cache->head_dim, batch, max_q, max_kv);
     const size_t rows = static_cast<size_t>(total) * hq;
     const size_t room = workspace == nullptr ? 0 : workspace_bytes / slice_bytes(rows, cache->head_dim);
     if (room < static_cast<size_t>(p.splits)) {
@@ -892,7 +921,8 @@ extern "C" size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, 
     if (cache == nullptr || cache->num_kv_heads <= 0 || !kv_head_dim_ok(cache->head_dim) || num_q_heads <= 0 ||
         num_q_heads % cache->num_kv_heads != 0 || batch <= 0 || max_q_len <= 0 || max_kv_len <= 0)
         return 0;
-    const Plan p = plan(cache->num_kv_heads, num_q_heads / cache->num_kv_heads, batch, max_q_len, max_kv_len);
+    const Plan p = plan(cache->num_kv_heads, num_q_heads / cache->num_kv_heads, cache->head_dim, batch,
+                        max_q_len, max_kv_len);
     if (p.splits <= 1) return 0;
     return p.splits * slice_bytes(static_cast<size_t>(batch) * max_q_len * num_q_heads, cache->head_dim);
 }
