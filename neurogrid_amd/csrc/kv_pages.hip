@@ -30,13 +30,14 @@ __device__ __forceinline__ N block_sum(N v, N* s) {
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x) / kWave; ++w) v += s[w];
+#pragma unroll
+    for (int w = 0; w < kPgThreads / kWave; ++w) v += s[w];
     __syncthreads();
     return v;
 }
 
-// Sum of v over the threads before this one.
-__device__ __forceinline__ int block_before(int v, int* s) {
+// Sum of v over the threads before this one; of all of them in *total.
+__device__ __forceinline__ int block_before(int v, int* s, int* total) {
     const int lane = threadIdx.x & 63;
     int x = v;
 #pragma unroll
@@ -46,17 +47,35 @@ __device__ __forceinline__ int block_before(int v, int* s) {
     }
     if (lane == 63) s[threadIdx.x >> 6] = x;
     __syncthreads();
-    int before = x - v;
-    for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) before += s[w];
+    int before = x - v, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kPgThreads / kWave; ++w) {
+        if (w < static_cast<int>(threadIdx.x >> 6)) before += s[w];
+        sum += s[w];
+    }
     __syncthreads();
+    *total = sum;
     return before;
 }
 
-// How many pages of [0, end) are used.
-__device__ __forceinline__ int used_before(const int* refs, int end, int* s) {
-    int n = 0;
-    for (int i = threadIdx.x; i < end; i += kPgThreads) n += refs[i] > 0;
-    return block_sum(n, s);
+// How many pages of [0, end) are used, and how many of [0, part), part <= end:
+// every block counts for itself (the counts stay in L2), 16 loads a thread on
+// their way at a time.
+__device__ __forceinline__ int used_before(const int* refs, int end, int part, unsigned long long* s, int* in_part) {
+    unsigned long long n = 0;  // both counts, end <= 2^30
+    for (int i0 = threadIdx.x; i0 < end; i0 += 16 * kPgThreads) {
+        int r[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) r[k] = refs[min(i0 + k * kPgThreads, end - 1)];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int i = i0 + k * kPgThreads;
+            if (i < end && r[k] > 0) n += 1ull + (i < part ? 1ull << 32 : 0);
+        }
+    }
+    n = block_sum(n, s);
+    *in_part = static_cast<int>(n >> 32);
+    return static_cast<int>(n & 0xffffffffull);
 }
 
 __device__ __forceinline__ int pages_of(int tokens, int ps_log2) {
@@ -89,24 +108,25 @@ __device__ __forceinline__ Growth growth(const PoolView& p, const int* old_lens,
 // LDS: the rank at which a row's pages start).
 __global__ __launch_bounds__(kPgThreads) void kv_grow_plan_kernel(PoolView p, const int* old_lens, const int* new_lens,
                                                                   int* copy_src, int* copy_dst, int* d_missing) {
-    __shared__ int first[kPgMaxRows + 1];
+    __shared__ int first[kPgMaxRows];
     __shared__ int s[kPgThreads / kWave];
-    __shared__ long long s_over[kPgThreads / kWave];
-    int at = 0;
-    long long over = 0;
+    __shared__ unsigned long long s_long[kPgThreads / kWave];
+    const int base = blockIdx.x * kPgThreads;
+    int need = 0;
+    unsigned long long over = 0;
     for (int r0 = 0; r0 < p.rows; r0 += kPgThreads) {
         const int r = r0 + threadIdx.x;
         const Growth g = r < p.rows ? growth(p, old_lens, new_lens, r) : Growth{0, 0, -1, 0};
-        const int need = g.want - g.have + (g.shared >= 0);
-        const int before = block_before(need, s);
-        if (r < p.rows) first[r] = at + before;
-        at += block_sum(need, s);
-        over += block_sum<long long>(g.missing, s_over);
+        int sum;
+        const int before = block_before(g.want - g.have + (g.shared >= 0), s, &sum);
+        if (r < p.rows) first[r] = need + before;
+        need += sum;
+        over += static_cast<unsigned>(g.missing);
     }
-    const int need = at;
-    const int free_all = p.pages - used_before(p.refs, p.pages, s);
-    const int missing = static_cast<int>(min(over + max(need - free_all, 0), 0x7fffffffll));
-    const int base = blockIdx.x * kPgThreads;
+    over = block_sum(over, s_long);
+    int here;
+    const int free_all = p.pages - used_before(p.refs, p.pages, base, s_long, &here);
+    const int missing = static_cast<int>(min(over + max(need - free_all, 0), 0x7fffffffull));
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) *d_missing = missing;
         for (int r = threadIdx.x; r < p.rows; r += kPgThreads) {
@@ -117,11 +137,12 @@ __global__ __launch_bounds__(kPgThreads) void kv_grow_plan_kernel(PoolView p, co
         }
     }
     if (missing != 0 || need == 0) return;
-    const int free_before = base - used_before(p.refs, base, s);
+    const int free_before = base - here;
     if (free_before >= need) return;
     const int page = base + threadIdx.x;
     const bool is_free = page < p.pages && p.refs[page] <= 0;
-    const int rank = free_before + block_before(is_free, s);
+    int sum;
+    const int rank = free_before + block_before(is_free, s, &sum);
     if (!is_free || rank >= need) return;
     int lo = 0, hi = p.rows - 1;  // the last row that starts at or before rank (rows that need nothing start with their successor)
     while (lo < hi) {
@@ -186,14 +207,15 @@ __global__ __launch_bounds__(256) void kv_free_kernel(PoolView p, const int* old
 __global__ __launch_bounds__(kPgThreads) void kv_compact_plan_kernel(PoolView p, int* copy_src, int* copy_dst,
                                                                      int capacity, int* d_moves) {
     __shared__ int s[kPgThreads / kWave];
+    __shared__ unsigned long long s_long[kPgThreads / kWave];
     const int base = blockIdx.x * kPgThreads;
-    const int n = used_before(p.refs, p.pages, s);
-    const int front = used_before(p.refs, n, s);  // used pages before n
+    int here, front, sum;
+    const int n = used_before(p.refs, p.pages, base, s_long, &here);
+    used_before(p.refs, n, n, s_long, &front);  // used pages before n
     const int moves = n - front;
-    const int here = used_before(p.refs, min(base, p.pages), s);
     const int page = base + threadIdx.x;
     const bool used = page < p.pages && p.refs[page] > 0;
-    const int before = here + block_before(used, s);
+    const int before = here + block_before(used, s, &sum);
     if (page < p.pages) {
         if (used && page >= n) copy_src[before - front] = page;
         if (!used && page < n) copy_dst[page - before] = page;
