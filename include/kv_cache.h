@@ -92,7 +92,8 @@ int ng_bf16_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const 
  * sequence are its last n tokens: query i stands at p = kv_len - n + i and sees
  * token j (0 <= j <= p) if window is 0, or j > p - window, or j < sinks:
  *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(softmax_scale q . k_j)
- * A query that sees nothing (p < 0, pages missing) gives 0. out may be q.
+ * A query that sees nothing (p < 0, pages missing) gives 0. out may be q, and
+ * must not overlap it otherwise.
  * With a workspace, long sequences are shared out over the GPU and joined by a
  * second launch. ng_kv_int8_attention_workspace says how many bytes that takes
  * for at most batch sequences of at most max_q_len queries and max_kv_len
@@ -100,7 +101,7 @@ int ng_bf16_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const 
  * shared out less, or not. Calls that overlap, and graphs that may, each need a
  * workspace of their own (16-byte aligned).
  * num_q_heads is a multiple of num_kv_heads; q and out are 16-byte aligned;
- * softmax_scale is finite and >= 0; window and sinks are >= 0. Scores, sums and
+ * softmax_scale is >= 0 and below FLT_MAX / log2(e); window and sinks are >= 0. Scores, sums and
  * the output are held in 32 bits; a weight times its page's V scale is rounded
  * to 11 bits, and to 2^-25 of the largest V scale that the query sees. */
 size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, int num_q_heads, int batch, int max_q_len,

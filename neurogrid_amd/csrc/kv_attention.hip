@@ -178,7 +178,9 @@ __device__ __forceinline__ float load_row(const uint16_t* row, bool real, At&& a
     }
 }
 
-// Few queries to a sequence: bound by reading the cache. A block of four waves
+// Few queries to a sequence: bound by reading the cache (64 sequences of up to
+// 4096 tokens, 32 heads on 8, D = 128: 63 us, 5.4 TB/s; one of 131071: 43 us, 6.2
+// TB/s, and 4-5 us for the join; 500 tokens: 6.4 us, latency). A block of four waves
 // takes up to 16 rows and a slice of the tokens; a wave every fourth tile of
 // 16 NB tokens, straight from memory into registers: K's codes of the next
 // tile are requested when this tile's are used up, then V's, so that half a
@@ -407,9 +409,11 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
     }
 }
 
-// Many queries to a sequence: bound by the matrix cores and the VALU, which
-// takes about 1.3 times as long for the conversions and the exponentials. A
-// block of four waves takes 128 rows, 32 a wave (32 x 32 x 16 MFMAs), and goes
+// Many queries to a sequence: bound by the power limit. 8192 tokens, 32 heads on
+// 8, D = 128, causal: 590-625 us on MI355X (880-930 TFLOP/s; a plain product
+// reaches 1090-1160 there) at 1.86 GHz, 468 us on zeros at full clock; without
+// the reads of first operands 552 of 596 us, without conversion into LDS 518,
+// without exponentials 551. A block of four waves takes 128 rows, 32 a wave (32 x 32 x 16 MFMAs), and goes
 // through tiles of 64 tokens. A tile's codes become fp16 once a block, on their
 // way into LDS: while a tile is multiplied, the next one's codes, which arrived
 // in registers a tile earlier, are converted into the other half of LDS, and
@@ -838,7 +842,7 @@ Plan plan(int hkv, int group, int D, int batch, int max_q, int max_kv) {
     const long long rows = static_cast<long long>(max_q) * group;
     p.prompt = rows >= kPromptFrom;
     p.row_tile = p.prompt ? kPromptRows : 16;
-    p.row_tiles = static_cast<int>((rows + p.row_tile - 1) / p.row_tile);
+    p.row_tiles = static_cast<int>(std::min((rows + p.row_tile - 1) / p.row_tile, 1ll << 30));
     const int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
     const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
     const long long want = (kBlocksWanted + blocks - 1) / blocks;
@@ -879,10 +883,15 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
     NG_REQUIRE(max_kv > 0, "%s: invalid max_kv_len %d", name, max_kv);
     NG_REQUIRE(hq > 0 && hq % cache->num_kv_heads == 0 && hq <= 32767,
                "%s: %d query heads on %d key/value heads", name, hq, cache->num_kv_heads);
-    NG_REQUIRE(__builtin_isfinite(scale) && scale >= 0.0f, "%s: softmax_scale must be finite and >= 0", name);
+    NG_REQUIRE(scale >= 0.0f && __builtin_isfinite(scale * 1.4426950408889634f),
+               "%s: softmax_scale must be >= 0 and below FLT_MAX / log2(e)", name);
     NG_REQUIRE(window >= 0 && sinks >= 0, "%s: window and sinks must be >= 0", name);
     NG_REQUIRE(aligned16(out) && aligned16(q) && aligned16(workspace), "%s: pointers must be 16-byte aligned", name);
     NG_REQUIRE(static_cast<long long>(total) * hq <= (1ll << 30), "%s: more than 2^30 query rows", name);
+    const size_t bytes = static_cast<size_t>(total) * hq * cache->head_dim * 2;
+    NG_REQUIRE(out == q || static_cast<char*>(out) + bytes <= static_cast<const char*>(q) ||
+                   static_cast<const char*>(q) + bytes <= static_cast<char*>(out),
+               "%s: out overlaps q without being q", name);
     max_q = std::min(max_q, total);
     AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
                total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,

@@ -56,12 +56,17 @@ def test_batches_that_are_refused(pre, capfd):
     # out, q, cache, cu, lens, table, batch, max_pages, total, max_q, max_kv, heads, scale, window, sinks, ws, bytes
     good = [P, P, c, P, P, P, 3, 4, 5, 6, 7, 4, 0.5, 0, 0, P, 64]
     bad = [(0, None), (1, None), (3, None), (4, None), (5, None), (6, 0), (6, 65536), (7, 0), (8, 0), (9, 0), (10, 0),
-           (11, 0), (11, 3), (11, 40000), (12, math.nan), (12, math.inf), (12, -0.5), (13, -1), (14, -1), (15, P + 4),
+           (11, 0), (11, 3), (11, 40000), (12, math.nan), (12, math.inf), (12, -0.5), (12, 3e38), (13, -1), (14, -1), (15, P + 4),
            (0, P + 4), (1, P + 2)]
     for i, x in bad:
         a = list(good)
         a[i] = x
         assert getattr(L, pre + "kv_int8_attention")(*a) == -1, (i, x)
+    for shift in (16, -16, 4 * 5 * 128 * 2 - 16):  # out inside q and q inside out
+        a = list(good)
+        a[0] = P + 65536 + shift
+        a[1] = P + 65536
+        assert getattr(L, pre + "kv_int8_attention")(*a) == -1, shift
     assert "neurogrid-amd: " + pre + "kv_int8_attention" in capfd.readouterr().err
 
 
@@ -114,6 +119,19 @@ def test_workspace_size_of_refused_arguments_is_zero():
     for a in ((0, 1, 1, 1000), (3, 1, 1, 1000), (8, 0, 1, 1000), (8, 1, 0, 1000), (8, 1, 1, 0)):
         assert L.ng_kv_int8_attention_workspace(c, *a) == 0
     assert L.ng_kv_int8_attention_workspace(C.byref(cache(head_dim=100)), 8, 1, 1, 100000) == 0
+
+
+def test_workspace_size():
+    """As many slices as blocks are wanted, and never more bytes than that many outputs; any hints are taken."""
+    L = _lib.load()
+    c = C.byref(cache(num_kv_heads=8))
+    row = 32 * (128 + 2) * 4  # a query's heads, fp32 outputs and (m, l)
+    assert L.ng_kv_int8_attention_workspace(c, 32, 1, 1, 500) == 0         # too short to share out
+    assert L.ng_kv_int8_attention_workspace(c, 32, 64, 1, 4096) == 0       # enough sequences
+    n = L.ng_kv_int8_attention_workspace(c, 32, 1, 1, 131071)
+    assert n % row == 0 and 32 <= n // row <= 64
+    for a in ((32, 65535, 1, 2 ** 31 - 1), (32, 1, 2 ** 31 - 1, 2 ** 31 - 1), (32, 2 ** 31 - 1, 2 ** 31 - 1, 1)):
+        assert L.ng_kv_int8_attention_workspace(c, *a) % row == 0
 
 
 # ---------------------------------------------------------------- the oracle
