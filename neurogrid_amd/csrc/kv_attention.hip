@@ -146,8 +146,8 @@ __device__ __forceinline__ float decay(float m, float to) {
 }
 
 // N pieces of 8 elements of a query row, piece j at row + at(j), as fp16
-// operands; `lanes` (16 or 32) and its doubles reach the lanes that hold the rest
-// of the row. Returns the factor that undoes bf16's scaling.
+// operands; the lanes FROM (16 or 32) and its doubles away hold the rest of the
+// row. Returns the factor that undoes bf16's scaling.
 template <typename T, int N, int FROM, typename At>
 __device__ __forceinline__ float load_row(const uint16_t* row, bool real, At&& at, f16x8 (&q)[N]) {
     u32x4 raw[N];
@@ -413,9 +413,9 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 // 8, D = 128, causal: 585-625 us on MI355X (880-940 TFLOP/s; a plain product
 // reaches 1090-1160 there) at 1.86 GHz, 468 us on zeros at full clock; without
 // the reads of first operands 552 of 596 us, without conversion into LDS 518,
-// without exponentials 551. A block of four waves takes 128 rows, 32 a wave (32 x 32 x 16 MFMAs), and goes
-// through tiles of 64 tokens. A tile's codes become fp16 once a block, on their
-// way into LDS: while a tile is multiplied, the next one's codes, which arrived
+// without exponentials 551. A block of four waves takes 128 rows, 32 a wave (32
+// x 32 x 16 MFMAs), and goes through tiles of 64 tokens. A tile's codes become
+// fp16 once a block, on their way into LDS: while a tile is multiplied, the next one's codes, which arrived
 // in registers a tile earlier, are converted into the other half of LDS, and
 // the one after that is requested. Wave w brings sub-block w.
 //   K in LDS: 16-byte pieces (d / 8, token), V: (sub-block, g, position of d),
@@ -828,9 +828,8 @@ size_t slice_bytes(size_t rows, int D) { return rows * (D + 2) * sizeof(float); 
 // token on sees half its tiles on average. (512 queries behind 8000 tokens, 8
 // heads: 178 us in one slice, 122 in two, 106 in four; a prompt of 1000, 32
 // heads: 31 us in one slice, 50 in two.)
-int prompt_splits(const Plan& p, int D, long long blocks, long long rows, int max_q, int tiles) {
+int prompt_splits(int D, long long blocks, long long rows, double average, int tiles) {
     const int resident = D <= 128 ? 512 : 256;
-    const double average = std::max(tiles - max_q / 128.0, tiles * 0.5);
     int best = 1;
     double least = 0.0;
     for (int s = 1; s <= 64 && s <= std::max(tiles / kTilesLeast, 1); ++s) {
@@ -846,17 +845,21 @@ int prompt_splits(const Plan& p, int D, long long blocks, long long rows, int ma
     return best;
 }
 
-Plan plan(int hkv, int group, int D, int batch, int max_q, int max_kv) {
+Plan plan(int hkv, int group, int D, int batch, int max_q, int max_kv, int window, int sinks) {
     Plan p;
     const long long rows = static_cast<long long>(max_q) * group;
     p.prompt = rows >= kPromptFrom;
     p.row_tile = p.prompt ? kPromptRows : 16;
     p.row_tiles = static_cast<int>(std::min((rows + p.row_tile - 1) / p.row_tile, 1ll << 30));
-    const int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
+    // Tiles that a block's rows see at most: all, or the window of each of its tokens and the first tokens.
+    int tiles = (std::min(max_kv, 1 << 30) + 63) / 64;
+    double average = std::max(tiles - max_q / 128.0, tiles * 0.5);
+    const long long seen = (static_cast<long long>(window) + p.row_tile / group + 127) / 64 + (static_cast<long long>(sinks) + 63) / 64;
+    if (window > 0 && seen < tiles) average = tiles = static_cast<int>(seen);
     const long long blocks = static_cast<long long>(batch) * hkv * p.row_tiles;
     const long long want = (kBlocksWanted + blocks - 1) / blocks;
     const int most = tiles < 4 * kTilesLeast ? 1 : tiles / kTilesLeast;
-    p.splits = p.prompt ? prompt_splits(p, D, blocks, rows * hkv * batch, max_q, tiles)
+    p.splits = p.prompt ? prompt_splits(D, blocks, rows * hkv * batch, average, tiles)
                         : static_cast<int>(std::min<long long>(want, most));
     p.chunk = (tiles + p.splits - 1) / p.splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
@@ -905,7 +908,7 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
     AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
                total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,
                16, 1, 1, static_cast<float*>(workspace)};
-    Plan p = plan(cache->num_kv_heads, a.group, cache->head_dim, batch, max_q, max_kv);
+    Plan p = plan(cache->num_kv_heads, a.group, cache->head_dim, batch, max_q, max_kv, a.window, sinks);
     const size_t rows = static_cast<size_t>(total) * hq;
     const size_t room = workspace == nullptr ? 0 : workspace_bytes / slice_bytes(rows, cache->head_dim);
     if (room < static_cast<size_t>(p.splits)) {
@@ -940,7 +943,7 @@ extern "C" size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, 
         num_q_heads % cache->num_kv_heads != 0 || batch <= 0 || max_q_len <= 0 || max_kv_len <= 0)
         return 0;
     const Plan p = plan(cache->num_kv_heads, num_q_heads / cache->num_kv_heads, cache->head_dim, batch,
-                        max_q_len, max_kv_len);
+                        max_q_len, max_kv_len, 0, 0);
     if (p.splits <= 1) return 0;
     return p.splits * slice_bytes(static_cast<size_t>(batch) * max_q_len * num_q_heads, cache->head_dim);
 }

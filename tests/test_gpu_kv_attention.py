@@ -94,6 +94,15 @@ def test_long_sequences_are_shared_out(lib):
     check(lib, 6, "bf16", 8, 8, 128, 16, [3] * 5, [5000, 2, 3, 4, 5], max_q=1)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_windows_in_long_sequences_are_shared_out(lib, new):
+    """A window that is a small part of the context, with first tokens, split and not."""
+    banner(f"kv attention window split new={new}")
+    for window, sinks in ((2000, 4), (1500, 700), (64, 5000)):
+        check(lib, 20, "f16", 8, 2, 128, 16, [new, new], [9000, 300], window, sinks)
+        check(lib, 20, "f16", 8, 2, 128, 16, [new, new], [9000, 300], window, sinks, workspace=None)
+
+
 def test_rows_that_see_nothing(lib):
     """No tokens, fewer tokens than queries, no page where the tokens should be: zeros, and never NaN."""
     banner("kv attention empty rows")
