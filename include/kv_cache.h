@@ -26,9 +26,9 @@ extern "C" {
 /* One layer's cache. A page holds page_size consecutive tokens of one
  * sequence for every head; k_codes and v_codes have num_pages * num_kv_heads *
  * page_size * head_dim bytes, k_scales and v_scales num_pages * num_kv_heads
- * floats ([page][head]). A value is code * scale of its page and head. The
- * order of the codes inside a page and head is the library's own
- * (ng_kv_int8_read gives them in order). head_dim is 64, 128, 192 or 256;
+ * floats ([page][head]): the largest magnitude of the page and head, a value
+ * being code * that / 127. The order of the codes inside a page and head is the
+ * library's own (ng_kv_int8_read gives them in order). head_dim is 64, 128, 192 or 256;
  * page_size 16, 32, 64 or 128; the code arrays are 16-byte aligned. */
 typedef struct {
     void* k_codes;
@@ -60,12 +60,13 @@ typedef struct {
  * cu_tokens[b + 1] - 1; context_lens [batch]: how many tokens the sequence
  * holds before, that is the position of the first new one; page_table
  * [batch, max_pages]. Per page and head, for K and V alike:
- *   m = largest finite |x| of the new tokens there; s = RN(m / 127), and the
- *   page's scale so far if it held tokens and that is larger;
- *   where s grew: old codes = rint(RN(code * RN(old scale / s)));
- *   new codes = clamp(rint(RN(x / s)), -127, 127), NaN as +127; 0 where s is 0.
- * What the cache holds is always finite. Codes behind a page's last token
- * become 0, and a page's scale while it held no token is not read. Two
+ *   m = largest finite |x| of the new tokens there, and of the page so far if it
+ *   held tokens;
+ *   where m grew: old codes = rint(code * old m / m);
+ *   new codes = rint(127 x / m), infinities +-127, NaN +127; 0 where m is 0.
+ * The quotients are exact before rint (ties to even). What the cache holds is
+ * always finite. Codes behind a page's last token become 0, and a page's
+ * magnitude while it held no token is not read. Two
  * sequences of a call must not write the same page. Tokens whose page is
  * missing (past max_pages or not a page's number) are not written; they are
  * counted into *d_dropped (device int, not cleared here; may be null). */
@@ -77,8 +78,8 @@ int ng_bf16_kv_int8_append(const ng_kv_int8_cache* cache, const void* k, const v
                            int total_tokens, int max_tokens, void* d_dropped);
 
 /* Reads tokens back: rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of k and v
- * [total_tokens, num_kv_heads, head_dim] become RN(code * scale) of sequence
- * b's tokens from position starts[b] on (fp16 or bf16). Tokens whose page is
+ * [total_tokens, num_kv_heads, head_dim] become RN(code * RN(m / 127)) of
+ * sequence b's tokens from position starts[b] on (fp16 or bf16). Tokens whose page is
  * missing read as 0; other rows are left as they are. */
 int ng_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const void* cu_tokens, const void* starts,
                     const void* page_table, int batch, int max_pages, int total_tokens, int max_tokens);
@@ -102,8 +103,11 @@ int ng_bf16_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const 
  * workspace of their own (16-byte aligned).
  * num_q_heads is a multiple of num_kv_heads; q and out are 16-byte aligned;
  * softmax_scale is >= 0 and below FLT_MAX / log2(e); window and sinks are >= 0. Scores, sums and
- * the output are held in 32 bits; a weight times its page's V scale is rounded
- * to 11 bits, and to 2^-25 of the largest V scale that the query sees. */
+ * the output are held in 32 bits. With more than 32 queries times heads of a
+ * group to a sequence (max_q_len), a weight times its page's V scale is rounded
+ * to 11 bits, and to 2^-25 of the largest V scale that the query sees; with
+ * fewer, to 22 bits and the same. A page whose V lies below 2^-126 (bf16's
+ * subnormals) may count as zeros. */
 size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, int num_q_heads, int batch, int max_q_len,
                                       int max_kv_len);
 int ng_kv_int8_attention(void* out, const void* q, const ng_kv_int8_cache* cache, const void* cu_q,

@@ -1,9 +1,10 @@
 // kv_attention.hip - attention over the 8-bit key/value cache (kv_cache.h; its
 // layout: kv_cache.hpp).
 //
-// With a page's scales k_s, v_s, codes k, v and x_j = c k_s (q . k_j):
-//   out = sum_j 2^(x_j - m) v_s v_j / sum_j 2^(x_j - m),  m a running maximum
-// of the visible x_j (c holds log2 e), sums in 32 bits. One pass over the cache.
+// With a page's magnitudes k_s, v_s, codes k, v and x_j = c k_s (q . k_j):
+//   out = 1/127 sum_j 2^(x_j - m) v_s v_j / sum_j 2^(x_j - m),  m a running
+// maximum of the visible x_j (c holds log2(e) / 127), sums in 32 bits. One pass
+// over the cache.
 //
 // Both products run on the matrix cores with the codes as exact fp16 integers:
 //   S^T = K Q^T: rows are tokens, columns queries; the scale of a token's page
@@ -12,7 +13,10 @@
 //     values of its second operand, so P goes from one product into the next
 //     without leaving its lane. P's entries are 2^(x - m) v_s / u, u the
 //     largest v_s that the row has met (the sums are rescaled when it grows, as
-//     they are when m does): at most 1, rounded to fp16 (11 bits) once.
+//     they are when m does): at most 1, as fp16. For single tokens, where memory
+//     is the bound, an entry's rounding error is a second fp16 entry (22 bits in
+//     all); prompts keep the first alone (11 bits), whose error is that of the
+//     output's own rounding at most.
 // The queries of all heads that share a key/value head, and of several tokens,
 // are the columns: row r of a sequence and key/value head is head r % group of
 // its token r / group.
@@ -32,14 +36,14 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kLeastUnit = 0x1p-126f;  // u of a row that has met nothing; its reciprocal is finite
+constexpr float kLeastUnit = 0x1p-124f;  // u of a row that has met nothing
 
 struct AttnArgs {
     const int* cu;
     const int* lens;
     const int* table;
     int max_pages, total, hq, group;
-    float scale;  // softmax_scale log2(e)
+    float scale;  // softmax_scale log2(e) / 127
     int window, sinks;
     int row_tile;       // rows that a block takes together
     int splits, chunk;  // slices of a sequence that there is room for; tiles of a slice
@@ -309,8 +313,9 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             const float base = mx == kNegInf ? 0.0f : mx;
             const float down = decay(m, mx);
             l *= down;
-            const float inv_u = __builtin_amdgcn_rcpf(un);
-            const float fade = un > u ? down * (u * inv_u) : down;
+            // 4 / u, so that neither u / 4 nor its reciprocal is subnormal, which v_rcp_f32 takes for 0.
+            const float inv_u = __builtin_amdgcn_rcpf(0.25f * un);
+            const float fade = un > u ? down * (0.25f * u * inv_u) : down;
             if (__any(fade != 1.0f)) {
 #pragma unroll
                 for (int c = 0; c < C; ++c)
@@ -319,10 +324,10 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             }
             m = mx;
             u = un;
-            uint32_t pp[NB][2];
+            uint32_t pp[NB][2], pl[NB][2];  // weights, and what their rounding left
 #pragma unroll
             for (int t = 0; t < NB; ++t) {
-                const float f = vs[t] * inv_u;
+                const float f = 0.25f * vs[t] * inv_u;
                 float w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -330,18 +335,24 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
                     l += w[e];
                     w[e] *= f;
                 }
-                pp[t][0] = pack2<f16>(w[0], w[1]);
-                pp[t][1] = pack2<f16>(w[2], w[3]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    pp[t][e] = pack2<f16>(w[2 * e], w[2 * e + 1]);
+                    pl[t][e] = pack2<f16>(w[2 * e] - el_get<f16, 0>(pp[t][e]), w[2 * e + 1] - el_get<f16, 1>(pp[t][e]));
+                }
             }
 #pragma unroll
             for (int t = 0; t < NB; t += 2) {
                 const f16x8 pb = __builtin_bit_cast(f16x8, u32x4{pp[t][0], pp[t][1], pp[t + 1][0], pp[t + 1][1]});
+                const f16x8 rest = __builtin_bit_cast(f16x8, u32x4{pl[t][0], pl[t][1], pl[t + 1][0], pl[t + 1][1]});
 #pragma unroll
                 for (int c = 0; c < C; ++c)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vr[t][c][j], vr[t + 1][c][j]), pb,
-                                                                           acc[c][j], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) {
+                        const f16x8 vt = codes8(vr[t][c][j], vr[t + 1][c][j]);
+                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, rest, acc[c][j], 0, 0, 0);
+                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pb, acc[c][j], 0, 0, 0);
+                    }
             }
             if (more) load_v(nsub);
 #pragma unroll
@@ -360,7 +371,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
         float L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kDecodeWaves; ++w) L += s_l[w][col] * decay(s_m[w][col], M);
-        const float f = decay(m, M) * u;
+        // u / (127 L) first: u times the sums may pass fp32's range where the output does not.
+        const float f = L == 0.0f ? 0.0f : decay(m, M) * (u / (127.0f * L));
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -370,7 +382,6 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
             }
         __syncthreads();
         if (wave == 0 && real) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             const size_t all = static_cast<size_t>(a.total) * a.hq;
             const size_t slot = blockIdx.x * all + row;
 #pragma unroll
@@ -381,7 +392,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 #pragma unroll
                     for (int w = 0; w < kDecodeWaves - 1; ++w) acc[c][j] += s_o[w][16 * c + 4 * kg + j][col];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * j + e] = acc[c][j][e] * inv;
+                    for (int e = 0; e < 4; ++e) o[4 * j + e] = acc[c][j][e];
                 }
                 if (sl.count > 1) {
                     float* to = a.part + slot * D + 64 * c + 16 * kg;
@@ -693,7 +704,7 @@ __global__ __launch_bounds__(kPromptWaves * kWave, D <= 128 ? 2 : 1) void kv_pro
         }
         l = with_half(l, plus);
         if (real) {
-            const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(lu) / l;
+            const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(lu) / (127.0f * l);
             const size_t all = static_cast<size_t>(a.total) * a.hq, slot = blockIdx.z * all + row;
             // acc[b][4 n + e] is position 32 b + 8 n + 4 g + e: i = 2 (b % 2) + n / 2, kg = 2 (n % 2) + g.
 #pragma unroll
@@ -906,7 +917,7 @@ int kv_attention(const char* name, void* out, const void* q, const ng_kv_int8_ca
                "%s: out overlaps q without being q", name);
     max_q = std::min(max_q, total);
     AttnArgs a{static_cast<const int*>(cu), static_cast<const int*>(lens), static_cast<const int*>(table), max_pages,
-               total, hq, hq / cache->num_kv_heads, scale * 1.4426950408889634f, std::min(window, 1 << 30), sinks,
+               total, hq, hq / cache->num_kv_heads, scale * static_cast<float>(1.4426950408889634 / 127.0), std::min(window, 1 << 30), sinks,
                16, 1, 1, static_cast<float*>(workspace)};
     Plan p = plan(cache->num_kv_heads, a.group, cache->head_dim, batch, max_q, max_kv, a.window, sinks);
     const size_t rows = static_cast<size_t>(total) * hq;

@@ -29,24 +29,63 @@ __device__ __forceinline__ uint32_t absmax_finite8(const u32x4 v, uint32_t m) {
     return m;
 }
 
-// 8 codes of x / s: the division-free form where every element is finite and s
-// is far from the ends of fp32's range (1 / s and the residual are then
-// normal), the IEEE quotient otherwise. Infinities saturate, NaN gives 127.
-template <typename T>
-__device__ __forceinline__ u32x2 kv_codes8(const u32x4 v, float s, float inv, bool fast) {
-    return fast ? qcode8<T>(v, inv, -s) : qcode8_div<T>(v, s);
+// A block's largest magnitude m as its codes are formed with it: 127 x / m is the
+// quotient of X = x (127 2^-e) and M = m 2^-e, 1 <= M < 2 (less for m below 2^-120).
+// x and m have at most 11 significant bits, so X is exact, and the quotient is a
+// half-integer or at least 2^-20 of itself away from one: RN(X / M) rounds to the
+// code that the real quotient has. It takes no division: with inv = RN(1 / M), z =
+// RN(X inv) is within a few ulp, the residual X - z M is exact, and one
+// correction step gives the correctly rounded quotient (Markstein).
+struct Block {
+    float scale;  // 127 2^-e
+    float m, inv; // M, RN(1 / M)
+    int e;
+};
+__device__ __forceinline__ Block block_of(float m) {
+    Block b;
+    b.e = max(static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23), 7) - 127;
+    b.scale = __builtin_ldexpf(127.0f, -b.e);
+    b.m = __builtin_ldexpf(m, -b.e);
+    b.inv = 1.0f / b.m;
+    return b;
+}
+__device__ __forceinline__ uint32_t code_bits(float x, const Block& b) {
+    const float z = x * b.inv;
+    return __builtin_bit_cast(uint32_t, fp32_barrier(__builtin_fmaf(__builtin_fmaf(z, -b.m, x), b.inv, z)) + kRoundMagic);
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+    const uint32_t lo = __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), hi = __builtin_amdgcn_perm(b3, b2, 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
-// rint(RN(code * r)) of four codes, 0 <= r <= 1.
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
-    uint32_t b[4];
+// Codes of the 8 elements of a vector. Where some are not finite, by the IEEE
+// quotient: infinities saturate, NaN gives 127.
+template <typename T>
+__device__ __forceinline__ u32x2 kv_codes8(const u32x4 v, const Block& b, bool finite) {
+    u32x2 out = {0, 0};
+    if (finite) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float q = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
-        b[e] = __builtin_bit_cast(uint32_t, fp32_barrier(q * r) + kRoundMagic);
+        for (int d = 0; d < 2; ++d)
+            out[d] = low_bytes(code_bits(el_mul<T, 0>(v[2 * d], b.scale), b), code_bits(el_mul<T, 1>(v[2 * d], b.scale), b),
+                               code_bits(el_mul<T, 0>(v[2 * d + 1], b.scale), b),
+                               code_bits(el_mul<T, 1>(v[2 * d + 1], b.scale), b));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = qclamp_ref(__builtin_rintf(to_f32<T>(lane16(v, e)) * b.scale / b.m));
+            out[e >> 2] |= (static_cast<uint32_t>(c) & 0xffu) << ((e & 3) * 8);
+        }
     }
-    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
-    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    return out;
+}
+
+// rint(code old / m) of four codes, old = the block's magnitude before times
+// 2^-e (the product is exact, so the code is again the real quotient's).
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, const Block& b) {
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = code_bits(fp32_barrier(static_cast<float>(static_cast<int8_t>(w >> (8 * e))) * old), b);
+    return low_bytes(c[0], c[1], c[2], c[3]);
 }
 
 // Grid: pages of a sequence (strided over), batch, 2 heads (K, V).
@@ -100,7 +139,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
         const bool has_old = wave * kSub < lo;  // of the wave's 16 tokens
 #pragma unroll
         for (int c = 0; c < C; ++c) old[c] = has_old ? ld16(mine + 1024 * c) ^ kKvBias : zero;
-        const float so = lo > 0 ? scales[ph] : 0.0f;
+        const float before = lo > 0 ? scales[ph] : 0.0f;
         uint32_t m = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) m = absmax_bits8(in[c][1], absmax_bits8(in[c][0], m));
@@ -118,24 +157,22 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
             __syncthreads();
             for (int w = 0; w < waves; ++w) m = umax32(m, s_max[w]);
         }
-        const float sn = to_f32<T>(static_cast<uint16_t>(m)) / 127.0f;
-        const float s = fmaxf(so, sn);
-        // Every wave of the block read the old scale before the barrier above,
-        // or is this wave.
-        if (threadIdx.x == 0) scales[ph] = s;
-        const bool grown = s > so;
+        const float now = fmaxf(before, to_f32<T>(static_cast<uint16_t>(m)));
+        // Every wave of the block read the old magnitude before the barrier
+        // above, or is this wave.
+        if (threadIdx.x == 0) scales[ph] = now;
+        const bool grown = now > before;
         if (wave * kSub + kSub <= lo && !grown) continue;  // old codes only, as they were
-        const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-        const float r = s > 0.0f ? so / s : 1.0f;
-        const bool fast = finite && s > 0x1p-100f && s < 0x1p100f;
+        const Block blk = block_of(now);
+        const float old_m = __builtin_ldexpf(before, -blk.e);
         // Which bytes of a dword are old tokens': all or none for K, by token for V.
         const int quad_old = min(max(lo - (wave * kSub + (t & ~3)), 0), 4);
         const uint32_t keep = is_v ? (quad_old == 4 ? ~0u : (1u << (8 * quad_old)) - 1u) : (slot < lo ? ~0u : 0u);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             u32x4 q = zero;
-            if (s > 0.0f) {
-                const u32x2 a = kv_codes8<T>(in[c][0], s, inv, fast), d = kv_codes8<T>(in[c][1], s, inv, fast);
+            if (now > 0.0f) {
+                const u32x2 a = kv_codes8<T>(in[c][0], blk, finite), d = kv_codes8<T>(in[c][1], blk, finite);
                 q = u32x4{a[0], a[1], d[0], d[1]};
             }
             if (is_v) {
@@ -145,7 +182,7 @@ __global__ __launch_bounds__(512) void kv_append_kernel(KvView kv, const uint16_
             if (has_old) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t o = grown ? rescale4(old[c][i], r) : old[c][i];
+                    const uint32_t o = grown ? rescale4(old[c][i], old_m, blk) : old[c][i];
                     q[i] = (o & keep) | (q[i] & ~keep);
                 }
             }
@@ -192,7 +229,7 @@ __global__ __launch_bounds__(512) void kv_read_kernel(KvView kv, uint16_t* k, ui
         u32x4 q[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) q[c] = there ? ld16(mine + 1024 * c) ^ kKvBias : u32x4{0, 0, 0, 0};
-        const float s = there ? load_uniform((is_v ? kv.vs : kv.ks) + ph) : 0.0f;
+        const float s = (there ? load_uniform((is_v ? kv.vs : kv.ks) + ph) : 0.0f) / 127.0f;
         uint16_t* row = x + static_cast<ptrdiff_t>(t0 + slot - start) * kv.hkv * D + 16 * kg;
 #pragma unroll
         for (int c = 0; c < C; ++c) {

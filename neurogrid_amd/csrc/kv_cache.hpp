@@ -25,7 +25,7 @@ constexpr uint32_t kKvBias = 0x80808080u;  // codes to bytes and back
 struct KvView {
     uint8_t* kc;
     uint8_t* vc;
-    float* ks;
+    float* ks;  // largest magnitudes; a value is code * that / 127
     float* vs;
     int num_pages, hkv, ps_log2;
 };

@@ -1,7 +1,9 @@
 """The 8-bit paged key/value cache, its page table and its attention in numpy: the checker of include/kv_cache.h.
 
-Quantisation is restated in fp32, operation by operation (codes and scales are
-compared bit for bit); attention in 64 bits; the page table in plain loops.
+Quantisation is restated with exact quotients (codes and scales are compared
+bit for bit); attention in 64 bits; the page table in plain loops. A cache's
+scales are the largest magnitudes of its pages and heads: a value is code *
+scale / 127.
 Codes are kept as [pages, heads, page_size, D] in token order; pack / unpack
 translate the library's order (its bytes hold code + 128).
 """
@@ -67,27 +69,27 @@ class Cache:
 
     def _block(self, pg, slot, x):
         H, page, D = self.codes.shape[1:]
-        mag = np.where(np.isfinite(x), np.abs(x), F(0)).max(axis=(0, 2))           # [H]
-        sn = (mag.astype(F) / F(127)).astype(F)
-        so = self.scales[pg].copy() if slot > 0 else np.zeros(H, F)
-        s = np.maximum(so, sn)
+        mag = np.where(np.isfinite(x), np.abs(x), F(0)).max(axis=(0, 2)).astype(F)   # [H]
+        old = self.scales[pg].copy() if slot > 0 else np.zeros(H, F)
+        s = np.maximum(old, mag)
+        # 127 x and code old are exact in 64 bits; their quotients by s are half-integers exactly, or further from one
+        # than a rounding of theirs (x and s have at most 11 significant bits).
         for h in range(H):
-            if slot > 0 and s[h] > so[h]:
-                r = F(so[h] / s[h])
-                q = self.codes[pg, h, :slot].astype(F) * r
+            m = np.float64(s[h])
+            if slot > 0 and s[h] > old[h]:
+                q = self.codes[pg, h, :slot].astype(np.float64) * np.float64(old[h]) / m
                 self.codes[pg, h, :slot] = np.rint(q).astype(np.int8)
             if s[h] > 0:
-                with np.errstate(invalid="ignore", over="ignore"):
-                    q = np.rint((x[:, h] / s[h]).astype(F))
-                q = np.where(np.isnan(q), F(127), np.clip(q, -127, 127))
+                q = np.rint(127 * x[:, h].astype(np.float64) / m)
+                q = np.where(np.isnan(q), 127, np.clip(q, -127, 127))
             else:
-                q = np.zeros((len(x), D), F)
+                q = np.zeros((len(x), D))
             self.codes[pg, h, slot:slot + len(x)] = q.astype(np.int8)
             self.codes[pg, h, slot + len(x):] = 0
         self.scales[pg] = s
 
     def read(self, cu, starts, table):
-        """Values in float32 (code * scale) of the tokens asked for, {row: [heads, D]}."""
+        """Values in float32 (code * RN(scale / 127)) of the tokens asked for, {row: [heads, D]}."""
         P, H, page, D = self.codes.shape
         out = {}
         for b in range(len(starts)):
@@ -95,7 +97,7 @@ class Cache:
                 col, slot = divmod(starts[b] + i, page)
                 pg = table[b, col] if col < table.shape[1] else -1
                 ok = 0 <= pg < P
-                out[cu[b] + i] = (self.codes[pg, :, slot].astype(F) * self.scales[pg][:, None] if ok
+                out[cu[b] + i] = (self.codes[pg, :, slot].astype(F) * (self.scales[pg] / F(127))[:, None] if ok
                                   else np.zeros((H, D), F))
         return out
 
@@ -117,8 +119,8 @@ def attention(q, kc: Cache, vc: Cache, cu, lens, table, scale, window=0, sinks=0
         pg = table[b, j // page] if L else np.zeros(0, int)
         there = (pg >= 0) & (pg < P)
         safe = np.where(there, pg, 0)
-        k = kc.codes[safe, :, j % page].astype(np.float64) * kc.scales[safe].astype(np.float64)[:, :, None]
-        v = vc.codes[safe, :, j % page].astype(np.float64) * vc.scales[safe].astype(np.float64)[:, :, None]
+        k = kc.codes[safe, :, j % page].astype(np.float64) * kc.scales[safe].astype(np.float64)[:, :, None] / 127
+        v = vc.codes[safe, :, j % page].astype(np.float64) * vc.scales[safe].astype(np.float64)[:, :, None] / 127
         for i in range(n):
             p = lens[b] - n + i
             seen = there & (j <= p)

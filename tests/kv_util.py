@@ -43,10 +43,10 @@ class DeviceCache:
 
 
 def random_cache(rng, pages, heads, page, D) -> tuple[K.Cache, K.Cache]:
-    """Full pages of codes and scales as a cache in use has them; scales over two decades."""
+    """Full pages of codes and scales as a cache in use has them; scales over one and a half decades."""
     def one():
         codes = np.clip(np.rint(rng.standard_normal((pages, heads, page, D)) * 40), -127, 127).astype(np.int8)
-        return K.Cache(codes, (10.0 ** rng.uniform(-2.5, -1.0, (pages, heads))).astype(np.float32))
+        return K.Cache(codes, (10.0 ** rng.uniform(-0.4, 1.1, (pages, heads))).astype(np.float32))
     return one(), one()
 
 

@@ -167,6 +167,20 @@ def test_bf16_queries_of_any_size(lib, gain):
     check(lib, 13, "bf16", 4, 2, 128, 16, [1, 40], [100, 90], scale=0.1 / gain if gain < 1e20 else 1e-31, gain=gain)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_bf16_values_at_the_ends_of_the_type(lib, new):
+    """Sums of values near 3e38 pass fp32's range, their mean does not; values near 1e-37 keep their precision."""
+    banner(f"kv attention bf16 V extremes new={new}")
+    for m in (3.38e38, 2e-37):
+        table, k, v, qb = problem(17, "bf16", 4, 2, 128, 16, [new] * 2, [500, 90])
+        used = np.unique(table[(table >= 0) & (table < len(k.scales))])
+        v.scales[used] = np.float32(m) * np.float32(0.9) ** (used[:, None] % 7)
+        cu = starts([new] * 2)
+        got = attend(lib, "bf16", DeviceCache(k, v), qb, cu, [500, 90], table, 0.05)
+        check_attention(got, "bf16", 128, K.attention(f32(qb, "bf16").reshape(qb.shape), k, v, cu, [500, 90], table,
+                                                      np.float32(0.05)))
+
+
 def test_scale_zero_is_the_mean(lib):
     banner("kv attention scale 0")
     check(lib, 14, "f16", 4, 2, 64, 16, [1, 30], [100, 30], scale=0.0)

@@ -144,6 +144,33 @@ def test_extreme_values(lib, dtype):
     assert all(np.isfinite(c.scales[table[0]]).all() for c in (k, v))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_ties_go_to_the_even_code(lib, dtype):
+    """Half-integer quotients: m / 2 for every significand of m (63.5 steps), a page of each, and codes that halve when
+    a louder token follows."""
+    banner(f"kv append ties {dtype}")
+    n = 11 if dtype == "f16" else 8
+    m = np.arange(2 ** (n - 1), 2 ** n, dtype=np.float64)
+    heads, D, page = 1, 64, 16
+    pages = len(m)
+    x = np.zeros((pages, page - 1, heads, D), np.float32)
+    x[:, 0, 0, 0], x[:, 0, 0, 1:4] = m, np.stack([m / 2, -m / 2, m / 4]).T
+    table = np.arange(pages, dtype=np.int32)[::-1].copy()[:, None]
+    k, v = fresh(rng_of(9), pages, heads, page, D)
+    dc = DeviceCache(k, v)
+    for part, at in ((x, 0), (np.full((pages, 1, heads, D), 1.0, np.float32) * 2 * m[:, None, None, None], page - 1)):
+        part = part.reshape(-1, heads, D)
+        cu = (np.arange(pages + 1) * (len(part) // pages)).astype(np.int32)
+        b = bits(part, dtype)
+        ctx = [at] * pages
+        for c in (k, v):
+            c.append(f32(b, dtype).reshape(b.shape), cu, ctx, table)
+        append(lib, dtype, dc, b, b, cu, ctx, table)
+        same(dc, k, v, f"at {at}")
+        if at == 0:
+            assert (k.codes[:, 0, 0, 1] == 64).all() and (k.codes[:, 0, 0, 2] == -64).all()
+
+
 def test_missing_pages_are_counted_and_nothing_else_is_touched(lib):
     banner("kv append missing pages")
     rng = rng_of(4)

@@ -153,13 +153,13 @@ def test_packing_is_a_permutation_and_its_formula():
 def test_append_by_hand():
     c = K.Cache(np.zeros((2, 1, 16, 64), np.int8), np.full((2, 1), np.nan, np.float32))
     x = np.zeros((2, 1, 64), np.float32)
-    x[0, 0, :3] = 127.0, -63.5, 0.5      # scale 1: 127, -64 (ties to even), 0
-    x[1, 0, 0] = 254.0                   # scale 2: the first token's codes halve
+    x[0, 0, :3] = 127.0, -63.5, 0.5      # a step of 1: 127, -64 (ties to even), 0
+    x[1, 0, 0] = 254.0                   # a step of 2: the first token's codes halve
     table = np.array([[1]], np.int32)
     assert c.append(x[:1], [0, 1], [0], table) == 0
-    assert list(c.codes[1, 0, 0, :3]) == [127, -64, 0] and c.scales[1, 0] == 1
+    assert list(c.codes[1, 0, 0, :3]) == [127, -64, 0] and c.scales[1, 0] == 127
     assert c.append(x[1:], [0, 1], [1], table) == 0
-    assert list(c.codes[1, 0, 0, :3]) == [64, -32, 0] and c.codes[1, 0, 1, 0] == 127 and c.scales[1, 0] == 2
+    assert list(c.codes[1, 0, 0, :3]) == [64, -32, 0] and c.codes[1, 0, 1, 0] == 127 and c.scales[1, 0] == 254
     assert c.append(x, [0, 2], [15], table) == 1  # one past the table
     assert np.isnan(c.scales[0, 0])
 
@@ -178,7 +178,7 @@ def test_append_is_within_half_a_step():
 def test_attention_of_the_oracle_by_hand():
     """Equal scores give the mean of what is seen; a score far above the others gives its value."""
     codes = np.zeros((1, 1, 16, 64), np.int8)
-    k, v = (K.Cache(codes.copy(), np.ones((1, 1), np.float32)) for _ in "kv")
+    k, v = (K.Cache(codes.copy(), np.full((1, 1), 127, np.float32)) for _ in "kv")
     v.codes[0, 0, :, 0] = np.arange(16)
     table = np.zeros((1, 1), np.int32)
     q = np.zeros((2, 1, 64))
