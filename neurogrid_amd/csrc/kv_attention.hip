@@ -183,8 +183,8 @@ __device__ __forceinline__ float load_row(const uint16_t* row, bool real, At&& a
 }
 
 // Few queries to a sequence: bound by reading the cache (64 sequences of up to
-// 4096 tokens, 32 heads on 8, D = 128: 63 us, 5.4 TB/s; one of 131071: 43 us, 6.2
-// TB/s, and 4-5 us for the join; 500 tokens: 6.4 us, latency). A block of four waves
+// 4096 tokens, 32 heads on 8, D = 128: 65 us, 5.3 TB/s; one of 131071: 44 us, 6.1
+// TB/s, and 4-5 us for the join; 500 tokens: 6.9 us, latency). A block of four waves
 // takes up to 16 rows and a slice of the tokens; a wave every fourth tile of
 // 16 NB tokens, straight from memory into registers: K's codes of the next
 // tile are requested when this tile's are used up, then V's, so that half a

@@ -11,7 +11,7 @@
 // A lane's two pieces of a row lie side by side and are two accesses: with
 // default-policy loads and stores the second meets the first's line in L2, with
 // non-temporal ones it did not. 4096 + 2920 + 1967 tokens of 8 heads, D = 128:
-// append 11.4 us (13.0 non-temporal; 38 MB), read 11.8 us (19.7).
+// append 11.7 us (13.0 non-temporal; 38 MB), read 11.6 us (19.7).
 // Bound: a token of a step is launch latency (4.1 us), prompts are HBM.
 #include "kv_cache.hpp"
 
