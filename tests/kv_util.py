@@ -101,15 +101,17 @@ def bound(dtype, D, ref):
     2^-24 of sum |q| |k|), times a factor of three roundings, with an exponential
     of an argument rounded to 2^-24 of at most 2 |x| log2 e, and of 2^-22 itself:
     relative error e of a weight. Weights enter the sum over V rounded to 11 bits
-    (2^-11 relative, 2^-25 of the largest where subnormal), times V's scale
-    factor (3 roundings), the sums over the tokens have a rounding a token. The
-    quotient doubles the weights' error. Then the output's own rounding.
+    (2^-11 relative; half of fp16's least step where subnormal, 2^-25, which is
+    2^-32 of the largest as weights stand at least 2^7 above their value, of a unit
+    that is at most twice the largest |v|), times V's scale factor (3 roundings),
+    the sums over the tokens have a rounding a token. The quotient doubles the
+    weights' error. Then the output's own rounding.
     """
     o, mag, dot, xmax, vmax, seen = ref
     u = 2.0 ** -24
     e = (D + 4) * u * dot + 8 * u * xmax + 2.0 ** -21
     half, least = HALF[dtype]
-    err = (2 * e)[:, None] * mag + (2.0 ** -11 + (2 * seen + 16) * u) * mag + (seen * 2.0 ** -25 * vmax)[:, None]
+    err = (2 * e)[:, None] * mag + (2.0 ** -11 + (2 * seen + 16) * u) * mag + (seen * 2.0 ** -31 * vmax)[:, None]
     return err * (1 + half) + half * np.abs(o) + least
 
 

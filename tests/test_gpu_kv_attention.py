@@ -160,6 +160,25 @@ def test_large_scores_and_uneven_scales(lib, dtype, new):
     check_attention(got, dtype, 128, K.attention(f32(qb, dtype).reshape(qb.shape), k, v, cu, kv, table, 1.0))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_many_small_weights_beside_a_large_one(lib, dtype, new):
+    """One token, whose value is 0, outweighs each of the others by 2^25.5: together they are the output."""
+    banner(f"kv attention small weights {dtype} {new}")
+    hq, hkv, D, page, n = 4, 1, 128, 16, 60000
+    table = np.arange(-(-n // page), dtype=np.int32)[None]
+    shape = (table.size, hkv, page, D)
+    rng = np.random.default_rng(8)
+    kc, vc = np.zeros(shape, np.int8), rng.integers(100, 128, shape).astype(np.int8)
+    kc[0, 0, 0], vc[0, 0, 0] = 127, 0
+    k, v = (K.Cache(c, np.full((table.size, hkv), m, np.float32)) for c, m in ((kc, 1.0), (vc, 3.0)))
+    qb = bits(np.ones((new, hq, D)), dtype)
+    scale = float(np.float32(25.5 * math.log(2) / D))
+    got = attend(lib, dtype, DeviceCache(k, v), qb, starts([new]), [n], table, scale, workspace=None)  # one slice
+    check_attention(got, dtype, D, K.attention(f32(qb, dtype).reshape(qb.shape), k, v, starts([new]), [n], table,
+                                               np.float32(scale)))
+
+
 @pytest.mark.parametrize("gain", [1e-6, 1e4, 1e30])
 def test_bf16_queries_of_any_size(lib, gain):
     """bf16 holds queries that fp16 cannot; the scale makes up for it."""
