@@ -20,7 +20,7 @@
 //     entry; prompts, where MFMAs are the bound, keep the first alone (11 bits).
 //     The error against 64 bits, relative (4 x 4096 tokens, fp16): 0.00028 with the
 //     first, 0.00021 with both, which is the output's own rounding; the second
-//     costs 2-4% of a single token's time (64 x 4096: 66.6 -> 67.8 us as a graph).
+//     costs 1.6-4.3% of a call's time (64 x 4096: 66.6 -> 67.8 us as a graph).
 // The queries of all heads that share a key/value head, and of several tokens,
 // are the columns: row r of a sequence and key/value head is head r % group of
 // its token r / group.
@@ -432,9 +432,9 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 // the reads of first operands 552 of 596 us, without conversion into LDS 518,
 // without exponentials 551. A block of four waves takes 128 rows, 32 a wave (32
 // x 32 x 16 MFMAs), and goes through tiles of 64 tokens. A tile's codes become
-// fp16 once a block, on their way into LDS: while a tile is multiplied, the next one's codes, which arrived
-// in registers a tile earlier, are converted into the other half of LDS, and
-// the one after that is requested. Wave w brings sub-block w.
+// fp16 once a block, on their way into LDS: while a tile is multiplied, the next
+// one's codes, which arrived in registers a tile earlier, are converted into the
+// other half of LDS, and the one after that is requested. Wave w brings sub-block w.
 //   K in LDS: 16-byte pieces (d / 8, token), V: (sub-block, g, position of d),
 //   a piece being the 8 tokens that lane half g of an MFMA's second operand
 //   holds, quads g and 2 + g. d = 64 c + 16 kg + 4 i + r stands at position
