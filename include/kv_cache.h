@@ -102,11 +102,11 @@ int ng_bf16_kv_int8_read(const ng_kv_int8_cache* cache, void* k, void* v, const 
  * shared out less, or not. Calls that overlap, and graphs that may, each need a
  * workspace of their own (16-byte aligned).
  * num_q_heads is a multiple of num_kv_heads; q and out are 16-byte aligned;
- * softmax_scale is >= 0 and below FLT_MAX / log2(e); window and sinks are >= 0. Scores, sums and
- * the output are held in 32 bits. With more than 32 queries times heads of a
- * group to a sequence (max_q_len), a weight times its page's V scale is rounded
- * to 11 bits, and to 2^-25 of the largest V scale that the query sees; with
- * fewer, to 22 bits and the same. A page whose V lies below 2^-126 (bf16's
+ * softmax_scale is >= 0 and below FLT_MAX / log2(e); window and sinks are >= 0.
+ * Scores, sums and the output are held in 32 bits. With more than 32 queries
+ * times heads of a group to a sequence (max_q_len), a weight times its page's V
+ * scale is rounded to 11 bits, and to 2^-32 of the largest V scale that the
+ * query sees; with fewer, to 22 bits and 2^-40. A page whose V lies below 2^-126 (bf16's
  * subnormals) may count as zeros. */
 size_t ng_kv_int8_attention_workspace(const ng_kv_int8_cache* cache, int num_q_heads, int batch, int max_q_len,
                                       int max_kv_len);
@@ -122,8 +122,8 @@ int ng_bf16_kv_int8_attention(void* out, const void* q, const ng_kv_int8_cache* 
 /* Copies page src[i] to page dst[i], codes and scales, for i < count in each of
  * the num_caches (1 .. 64) caches, which must agree in their sizes (a host array:
  * one per layer). Pairs with a page number outside [0, num_pages) are skipped
- * (-1: nothing to copy). No page may be the destination of two pairs, or of one
- * and the source of another. */
+ * (-1: nothing to copy); count is at most 2^30. No page may be the destination
+ * of two pairs, or of one and the source of another. */
 int ng_kv_int8_copy_pages(const ng_kv_int8_cache* caches, int num_caches, const void* src, const void* dst,
                           int count);
 
@@ -159,7 +159,7 @@ int ng_kv_pages_free(const ng_kv_pages* pages, const void* old_lens, const void*
  * refs and every entry of table follow; copy_src[k], copy_dst[k] say what to
  * copy (in every layer, before the pages are next used), -1 behind the last
  * move; *d_moves becomes the number of moves. capacity, the ints that
- * copy_src and copy_dst have, is at least num_pages / 2. */
+ * copy_src and copy_dst have, is at least num_pages / 2 and at most 2^30. */
 int ng_kv_pages_compact(const ng_kv_pages* pages, void* copy_src, void* copy_dst, int capacity, void* d_moves);
 
 #ifdef __cplusplus

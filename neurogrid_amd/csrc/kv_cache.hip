@@ -387,6 +387,7 @@ extern "C" int ng_kv_int8_copy_pages(const ng_kv_int8_cache* caches, int num_cac
     NG_REQUIRE(caches && src && dst, "%s: null pointer", name);
     NG_REQUIRE(num_caches >= 1 && num_caches <= 64, "%s: %d caches are outside 1..64", name, num_caches);
     NG_REQUIRE(count > 0, "%s: invalid count %d", name, count);
+    NG_REQUIRE(count <= (1 << 30), "%s: count %d is above 2^30", name, count);
     for (int i = 0; i < num_caches; ++i) {
         if (kv_check_cache(name, &caches[i]) != 0) return -1;
         NG_REQUIRE(caches[i].num_pages == caches[0].num_pages && caches[i].num_kv_heads == caches[0].num_kv_heads &&

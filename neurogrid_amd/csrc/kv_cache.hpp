@@ -58,7 +58,8 @@ inline int kv_check_batch(const char* name, const ng_kv_int8_cache* c, const voi
     NG_REQUIRE(batch > 0 && batch <= 65535, "%s: batch %d is outside 1..65535", name, batch);
     NG_REQUIRE(max_pages > 0 && total > 0 && most > 0, "%s: invalid sizes (max_pages=%d, tokens=%d, longest=%d)", name,
                max_pages, total, most);
-    NG_REQUIRE(total <= (1 << 30) && max_pages <= (1 << 30) / c->page_size, "%s: more than 2^30 tokens", name);
+    NG_REQUIRE(total < (1 << 30), "%s: 2^30 tokens or more", name);
+    NG_REQUIRE(max_pages <= (1 << 30) / c->page_size, "%s: a table of more than 2^30 tokens", name);
     return 0;
 }
 

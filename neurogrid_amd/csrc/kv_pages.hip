@@ -325,6 +325,7 @@ extern "C" int ng_kv_pages_compact(const ng_kv_pages* pages, void* copy_src, voi
     NG_REQUIRE(copy_src && copy_dst && d_moves, "%s: null pointer", name);
     NG_REQUIRE(capacity >= pages->num_pages / 2 && capacity > 0, "%s: capacity %d is below num_pages / 2 = %d", name,
                capacity, pages->num_pages / 2);
+    NG_REQUIRE(capacity <= (1 << 30), "%s: capacity %d is above 2^30", name, capacity);
     const PoolView p = pool_view(*pages);
     int *cs = static_cast<int*>(copy_src), *cd = static_cast<int*>(copy_dst), *mv = static_cast<int*>(d_moves);
     kv_compact_plan_kernel<<<dim3(page_blocks(p.pages)), dim3(kPgThreads), 0, stream()>>>(p, cs, cd, capacity, mv);

@@ -209,3 +209,31 @@ def test_page_table_of_the_oracle_keeps_its_counts():
             assert (np.diff((refs > 0).astype(int)) <= 0).all()
         assert (refs == np.bincount(table[table >= 0], minlength=pages)).all()
         assert ((table >= 0).sum(1) == -(-lens // page)).all()
+
+
+# Without a device a launch is an error too: what is refused is told by its message.
+
+def test_a_compactions_lists_are_at_most_2_30(capfd):
+    """The kernel's index goes a stride past the capacity: it would wrap and never end."""
+    L = _lib.load()
+    p = C.byref(KVPages(P, P, 4, 4, 16, 16))
+    for n in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert L.ng_kv_pages_compact(p, P, P, n, P) == -1
+        assert f"ng_kv_pages_compact: capacity {n} is above 2^30" in capfd.readouterr().err
+
+
+def test_page_copies_are_at_most_2_30(capfd):
+    """The kernel's index goes a stride past the count: it would wrap, below the lists."""
+    L = _lib.load()
+    for n in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert L.ng_kv_int8_copy_pages(C.byref(cache()), 1, P, P, n) == -1
+        assert f"ng_kv_int8_copy_pages: count {n} is above 2^30" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("pre", ["ng_", "ng_bf16_"])
+def test_a_batch_is_below_2_30_tokens(pre, capfd):
+    """A start of 2^30 and as many rows would end at 2^31."""
+    L = _lib.load()
+    for total in (2 ** 30, 2 ** 30 + 1):
+        assert getattr(L, pre + "kv_int8_read")(C.byref(cache()), P, P, P, P, P, 3, 4, total, 6) == -1
+        assert "kv_int8_read: 2^30 tokens or more" in capfd.readouterr().err
