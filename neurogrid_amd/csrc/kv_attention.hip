@@ -427,7 +427,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void kv_decode_kernel(uint16_
 }
 
 // Many queries to a sequence: bound by the power limit. 8192 tokens, 32 heads on
-// 8, D = 128, causal: 585-625 us on MI355X (880-940 TFLOP/s; a plain product
+// 8, D = 128, causal: 570-625 us on MI355X (880-965 TFLOP/s; a plain product
 // reaches 1090-1160 there) at 1.86 GHz, 468 us on zeros at full clock; without
 // the reads of first operands 552 of 596 us, without conversion into LDS 518,
 // without exponentials 551. A block of four waves takes 128 rows, 32 a wave (32

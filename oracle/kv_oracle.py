@@ -1,4 +1,4 @@
-"""The 8-bit paged key/value cache, its page table and its attention in numpy: the checker of include/kv_cache.h.
+"""The 8-bit paged key/value cache, its page table and its attention in numpy: the oracle of include/kv_cache.h.
 
 Quantisation is restated with exact quotients (codes and scales are compared
 bit for bit); attention in 64 bits; the page table in plain loops. A cache's
